@@ -71,9 +71,9 @@ const char* pa_status_string(int status);
 
 /* ABI version this header describes (major * 100 + minor). 101: the append,
  * RoPE + append, fused QKV and cascade-plan calls take the number of page ids
- * (num_kv_indices) after kv_indptr. A caller built against another version
- * must refuse the library (the Python binding does). */
-#define PA_ABI_VERSION 101
+ * (num_kv_indices) after kv_indptr. 102: the pa_window_* calls. A caller built
+ * against another version must refuse the library (the Python binding does). */
+#define PA_ABI_VERSION 102
 
 /* ABI version of this library (major * 100 + minor); equals PA_ABI_VERSION
  * of the header it was built from. */
@@ -270,6 +270,46 @@ int pa_decode_append_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
                          void* workspace, size_t workspace_bytes, void* out, float* lse,
                          void* stream);
 
+/* Sliding-window decode with sinks (FlashInfer's window_left; the reference
+ * attends full contexts, src/models/llama.py:230-245). Request b's query is
+ * at position kv_len - 1 and sees key j iff
+ *   kv_len - 1 - j <= window_left  or  j < num_sink_tokens.
+ * window_left >= 0 (0: the query's own key and the sinks). Pages without a
+ * visible key are not read, nor are their entries of kv_indices, which may
+ * hold anything (pages given back to the pool, -1). The plan copies the
+ * visible page ids into the workspace; num_kv_indices, window_left and
+ * num_sink_tokens of the run calls are the plan's. kv_len = 0 gives a zero
+ * row and LSE -inf. Other arguments as for pa_decode_plan / pa_decode_run /
+ * pa_decode_append_run; a position of the append call may lie in a page that
+ * is not visible: the pool slot is written all the same. */
+size_t pa_window_decode_workspace_bytes(int32_t batch_size, int64_t num_kv_indices,
+                                        int32_t num_qo_heads, int32_t num_kv_heads,
+                                        int32_t head_dim, int32_t window_left,
+                                        int32_t num_sink_tokens);
+int pa_window_decode_plan(const int32_t* kv_indptr, const int32_t* kv_indices,
+                          const int32_t* kv_last_page_len, int32_t batch_size,
+                          int64_t num_kv_indices, int32_t num_qo_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t page_size, int32_t window_left,
+                          int32_t num_sink_tokens, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int pa_window_decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                         const pa_kv_cache* cache, const int32_t* kv_indices,
+                         const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                         int32_t batch_size, int64_t num_kv_indices, int32_t num_qo_heads,
+                         int32_t window_left, int32_t num_sink_tokens, float sm_scale,
+                         void* workspace, size_t workspace_bytes, void* out, float* lse,
+                         void* stream);
+int pa_window_decode_append_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                                const void* append_key, int64_t key_stride_n,
+                                int64_t key_stride_h, const void* append_value,
+                                int64_t value_stride_n, int64_t value_stride_h,
+                                const int32_t* positions, const pa_kv_cache* cache,
+                                const int32_t* kv_indices, const int32_t* kv_indptr,
+                                const int32_t* kv_last_page_len, int32_t batch_size,
+                                int64_t num_kv_indices, int32_t num_qo_heads, int32_t window_left,
+                                int32_t num_sink_tokens, float sm_scale, void* workspace,
+                                size_t workspace_bytes, void* out, float* lse, void* stream);
+
 /* Two-level (cascade) decode, FlashInfer's MultiLevelCascadeAttentionWrapper
  * with two levels, for a batch whose requests all begin with the same shared
  * prefix pages — what the reference's RadixCache produces when requests share
@@ -342,6 +382,29 @@ int pa_prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const 
                    const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
                    int32_t num_qo_heads, int32_t causal, float sm_scale, void* workspace,
                    size_t workspace_bytes, void* out, float* lse, void* stream);
+
+/* Sliding-window prefill with sinks: row i of a request with qo_len rows and
+ * kv_len keys is at position p = kv_len - qo_len + i and sees key j iff
+ *   (p - j <= window_left or j < num_sink_tokens) and (j <= p or !causal).
+ * Pages that none of a request's rows sees are not read, nor are their page
+ * ids (see pa_window_decode_plan). Plan and run take the same window;
+ * workspace as for pa_prefill_plan (pa_prefill_workspace_bytes). Rows of one
+ * work item (256 / (H_q / H_kv) consecutive queries) share K / V tiles: a
+ * value that is not finite reaches every row of an item that one of its rows
+ * sees it from, as in pa_prefill_run. */
+int pa_window_prefill_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
+                           const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
+                           int64_t num_kv_indices, int32_t num_qo_heads, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t page_size, int32_t window_left,
+                           int32_t num_sink_tokens, void* workspace, size_t workspace_bytes,
+                           void* stream);
+int pa_window_prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                          const pa_kv_cache* cache, const int32_t* qo_indptr,
+                          const int32_t* kv_indices, const int32_t* kv_indptr,
+                          const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
+                          int32_t num_qo_heads, int32_t causal, int32_t window_left,
+                          int32_t num_sink_tokens, float sm_scale, void* workspace,
+                          size_t workspace_bytes, void* out, float* lse, void* stream);
 
 /* Replaces flashinfer.merge_states (the split-KV log-sum-exp merge):
  * v [seq_len, num_states, num_heads, D] (dtype), s [seq_len, num_states,

@@ -33,7 +33,7 @@ PA_NOALLOC_SCRATCH_BYTES = 24 * 1024 * 1024
 
 # PA_ABI_VERSION of include/paged_attn.h that SIGNATURES mirrors; a library
 # reporting another version is refused (argument lists would not line up).
-ABI_VERSION = 101
+ABI_VERSION = 102
 
 
 class PagedKVCache(ctypes.Structure):
@@ -117,6 +117,36 @@ SIGNATURES = {
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
          c_void_p, POINTER(PagedKVCache), c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_float,
          c_void_p, c_size_t, c_void_p, c_void_p, c_void_p],
+    ),
+    "pa_window_decode_workspace_bytes": (
+        c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "pa_window_decode_plan": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
+         c_int32, c_int32, c_void_p, c_size_t, c_void_p],
+    ),
+    "pa_window_decode_run": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, POINTER(PagedKVCache), c_void_p, c_void_p, c_void_p, c_int32,
+         c_int64, c_int32, c_int32, c_int32, c_float, c_void_p, c_size_t, c_void_p, c_void_p,
+         c_void_p],
+    ),
+    "pa_window_decode_append_run": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+         c_void_p, POINTER(PagedKVCache), c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32,
+         c_int32, c_int32, c_float, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p],
+    ),
+    "pa_window_prefill_plan": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32,
+         c_int32, c_int32, c_int32, c_void_p, c_size_t, c_void_p],
+    ),
+    "pa_window_prefill_run": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, POINTER(PagedKVCache), c_void_p, c_void_p, c_void_p,
+         c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p,
+         c_size_t, c_void_p, c_void_p, c_void_p],
     ),
     "pa_cascade_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "pa_cascade_plan": (

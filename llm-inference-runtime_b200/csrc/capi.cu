@@ -18,6 +18,7 @@
 #include "tables.cuh"
 #include "qkv.cuh"
 #include "cascade.cuh"
+#include "window.cuh"
 
 namespace {
 
@@ -200,20 +201,33 @@ size_t decode_ws_bytes(const DecodePlanShape& s, int batch, int hkv, int head_di
   return decode_ws_layout(s.units, batch, hkv, head_dim, s.g.hb).total;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kWindow = false>
 int launch_decode(const CUtensorMap& km, const CUtensorMap& vm, const DecodeParams& prm,
                   const DecodePlanShape& sh, int dev, cudaStream_t stream) {
   // Largest dynamic shared memory already allowed for this kernel, per device.
   static std::atomic<int> allowed[kMaxDevices];
   if (dev < 0 || dev >= kMaxDevices) return PA_ERR_CUDA;
   if (allowed[dev].load(std::memory_order_relaxed) < sh.g.smem_bytes) {
-    if (cudaFuncSetAttribute(decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(decode_kernel<T, D, kWindow>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
                              sh.g.smem_bytes) != cudaSuccess)
       return PA_ERR_CUDA;
     allowed[dev].store(sh.g.smem_bytes, std::memory_order_relaxed);
   }
-  return launch_chain(decode_kernel<T, D>, dim3(sh.ctas), dim3(sh.g.threads), sh.g.smem_bytes,
-                      stream, km, vm, prm);
+  return launch_chain(decode_kernel<T, D, kWindow>, dim3(sh.ctas), dim3(sh.g.threads),
+                      sh.g.smem_bytes, stream, km, vm, prm);
+}
+
+template <bool kWindow>
+int launch_decode_any(int dtype, int head_dim, const CUtensorMap& km, const CUtensorMap& vm,
+                      const DecodeParams& prm, const DecodePlanShape& sh, int dev,
+                      cudaStream_t stream) {
+  if (dtype == PA_DTYPE_BF16)
+    return head_dim == 64
+               ? launch_decode<__nv_bfloat16, 64, kWindow>(km, vm, prm, sh, dev, stream)
+               : launch_decode<__nv_bfloat16, 128, kWindow>(km, vm, prm, sh, dev, stream);
+  return head_dim == 64 ? launch_decode<__half, 64, kWindow>(km, vm, prm, sh, dev, stream)
+                        : launch_decode<__half, 128, kWindow>(km, vm, prm, sh, dev, stream);
 }
 
 // 3-D map over q [tokens, heads, dim] (strides in elements), box (64 dims,
@@ -237,20 +251,33 @@ int encode_q_map(CUtensorMap* map, const void* q, int64_t stride_n, int64_t stri
   return r == CUDA_SUCCESS ? PA_OK : PA_ERR_INVALID_ARGUMENT;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kWindow = false>
 int launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
                    const CUtensorMap& om, const PrefillParams& prm, int64_t grid, int dev,
                    cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   constexpr int smem = PfCfg<D>::kSmemBytes;
-  if (allow_smem(prefill_kernel<T, D>, smem, &done, dev) != cudaSuccess) return PA_ERR_CUDA;
+  if (allow_smem(prefill_kernel<T, D, kWindow>, smem, &done, dev) != cudaSuccess)
+    return PA_ERR_CUDA;
   if (grid <= 0) return PA_OK;
   // persistent: one CTA per SM at most, each taking items until none is left
   const int sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
   grid = std::min<int64_t>(grid, sms);
-  prefill_kernel<T, D><<<static_cast<unsigned>(grid), kPfThreads, smem, stream>>>(qm, km, vm, om,
-                                                                                  prm);
+  prefill_kernel<T, D, kWindow>
+      <<<static_cast<unsigned>(grid), kPfThreads, smem, stream>>>(qm, km, vm, om, prm);
   return launch_status();
+}
+
+template <bool kWindow>
+int launch_prefill_any(int dtype, int head_dim, const CUtensorMap& qm, const CUtensorMap& km,
+                       const CUtensorMap& vm, const CUtensorMap& om, const PrefillParams& prm,
+                       int64_t grid, int dev, cudaStream_t s) {
+  if (dtype == PA_DTYPE_BF16)
+    return head_dim == 64
+               ? launch_prefill<__nv_bfloat16, 64, kWindow>(qm, km, vm, om, prm, grid, dev, s)
+               : launch_prefill<__nv_bfloat16, 128, kWindow>(qm, km, vm, om, prm, grid, dev, s);
+  return head_dim == 64 ? launch_prefill<__half, 64, kWindow>(qm, km, vm, om, prm, grid, dev, s)
+                        : launch_prefill<__half, 128, kWindow>(qm, km, vm, om, prm, grid, dev, s);
 }
 
 }  // namespace
@@ -766,11 +793,19 @@ struct DecodeAppend {
   const int32_t* pos_base;  // device word subtracted from each position, or nullptr
 };
 
+// Sliding-window plan handed to decode_run (nullptr: full contexts). The
+// table arguments of decode_run are then the plan's compacted table.
+struct DecodeWindow {
+  const int4* window;
+  const int32_t* table_indptr;
+  const int32_t* table_indices;
+};
+
 int decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_kv_cache* cache,
                const int32_t* kv_indices, const int32_t* kv_indptr,
                const int32_t* kv_last_page_len, int32_t batch_size, int32_t num_qo_heads,
                float sm_scale, void* workspace, size_t workspace_bytes, void* out, float* lse,
-               void* stream, const DecodeAppend* app) {
+               void* stream, const DecodeAppend* app, const DecodeWindow* win = nullptr) {
   int st = check_cache(cache);
   if (st != PA_OK) return st;
   if (q == nullptr || out == nullptr || kv_indices == nullptr || kv_indptr == nullptr ||
@@ -822,6 +857,9 @@ int decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_k
   p.counter = reinterpret_cast<int32_t*>(ws + L.counter);
   p.part_lse = reinterpret_cast<float*>(ws + L.part_lse);
   p.part_o = reinterpret_cast<float*>(ws + L.part_o);
+  p.window = win != nullptr ? win->window : nullptr;
+  p.table_indptr = win != nullptr ? win->table_indptr : nullptr;
+  p.table_indices = win != nullptr ? win->table_indices : nullptr;
   p.append_pos = nullptr;
   p.append_pos_base = nullptr;
   p.new_k = p.new_v = nullptr;
@@ -847,11 +885,8 @@ int decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_k
     p.pool_token_stride = cache->token_stride * esz;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache->dtype == PA_DTYPE_BF16)
-    return D == 64 ? launch_decode<__nv_bfloat16, 64>(km, vm, p, sh, dev, s)
-                   : launch_decode<__nv_bfloat16, 128>(km, vm, p, sh, dev, s);
-  return D == 64 ? launch_decode<__half, 64>(km, vm, p, sh, dev, s)
-                 : launch_decode<__half, 128>(km, vm, p, sh, dev, s);
+  return win != nullptr ? launch_decode_any<true>(cache->dtype, D, km, vm, p, sh, dev, s)
+                        : launch_decode_any<false>(cache->dtype, D, km, vm, p, sh, dev, s);
 }
 
 }  // namespace
@@ -889,6 +924,130 @@ int pa_decode_append_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
                     stream, &app);
 }
 
+size_t pa_window_decode_workspace_bytes(int32_t batch_size, int64_t num_kv_indices,
+                                        int32_t num_qo_heads, int32_t num_kv_heads,
+                                        int32_t head_dim, int32_t window_left,
+                                        int32_t num_sink_tokens) {
+  (void)num_qo_heads;
+  const int dev = current_device();
+  if (dev < 0 || batch_size < 0 || num_kv_indices < 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      window_left < 0 || num_sink_tokens < 0)
+    return 0;
+  DecodePlanShape sh;
+  if (!decode_shape(dev, num_kv_heads, head_dim, &sh)) return 0;
+  return window_decode_ws_layout(batch_size, num_kv_indices, window_left, num_sink_tokens, kPage,
+                                 decode_ws_bytes(sh, batch_size, num_kv_heads, head_dim))
+      .total;
+}
+
+int pa_window_decode_plan(const int32_t* kv_indptr, const int32_t* kv_indices,
+                          const int32_t* kv_last_page_len, int32_t batch_size,
+                          int64_t num_kv_indices, int32_t num_qo_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t page_size, int32_t window_left,
+                          int32_t num_sink_tokens, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  if (kv_indptr == nullptr || kv_last_page_len == nullptr || workspace == nullptr ||
+      (num_kv_indices > 0 && kv_indices == nullptr))
+    return PA_ERR_INVALID_ARGUMENT;
+  if (batch_size <= 0 || num_kv_indices < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 ||
+      window_left < 0 || num_sink_tokens < 0)
+    return PA_ERR_INVALID_ARGUMENT;
+  if (num_qo_heads % num_kv_heads) return PA_ERR_INVALID_ARGUMENT;
+  if (num_qo_heads / num_kv_heads > kMaxGroup) return PA_ERR_UNSUPPORTED;
+  if (head_dim != 64 && head_dim != 128) return PA_ERR_UNSUPPORTED;
+  if (page_size != kPage) return PA_ERR_UNSUPPORTED;
+  if (!aligned16(workspace)) return PA_ERR_INVALID_ARGUMENT;
+  const int dev = current_device();
+  DecodePlanShape sh;
+  if (!decode_shape(dev, num_kv_heads, head_dim, &sh))
+    return dev < 0 ? PA_ERR_CUDA : PA_ERR_UNSUPPORTED;
+  const WindowDecodeWsLayout L =
+      window_decode_ws_layout(batch_size, num_kv_indices, window_left, num_sink_tokens, page_size,
+                              decode_ws_bytes(sh, batch_size, num_kv_heads, head_dim));
+  if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
+  const int copiers = std::min(batch_size, sh.ctas - 1);
+  return launch_chain(window_decode_plan_kernel, dim3(1 + copiers), dim3(kWindowPlanThreads), 0,
+                      static_cast<cudaStream_t>(stream), kv_indptr, kv_last_page_len, kv_indices,
+                      num_kv_indices, batch_size, num_kv_heads, num_qo_heads, head_dim, page_size,
+                      window_left, num_sink_tokens, sh.units, sh.g.hb, /*min_per_group=*/4,
+                      static_cast<uint8_t*>(workspace), L);
+}
+
+}  // extern "C"
+
+namespace {
+
+int window_decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                      const pa_kv_cache* cache, const int32_t* kv_indices,
+                      const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                      int32_t batch_size, int64_t num_kv_indices, int32_t num_qo_heads,
+                      int32_t window_left, int32_t num_sink_tokens, float sm_scale,
+                      void* workspace, size_t workspace_bytes, void* out, float* lse, void* stream,
+                      const DecodeAppend* app) {
+  const int st = check_cache(cache);
+  if (st != PA_OK) return st;
+  if (kv_indices == nullptr || kv_indptr == nullptr || workspace == nullptr)
+    return PA_ERR_INVALID_ARGUMENT;
+  if (batch_size <= 0 || num_kv_indices < 0 || window_left < 0 || num_sink_tokens < 0)
+    return PA_ERR_INVALID_ARGUMENT;
+  if (cache->head_dim != 64 && cache->head_dim != 128) return PA_ERR_UNSUPPORTED;
+  const int dev = current_device();
+  DecodePlanShape sh;
+  if (!decode_shape(dev, cache->num_kv_heads, cache->head_dim, &sh))
+    return dev < 0 ? PA_ERR_CUDA : PA_ERR_UNSUPPORTED;
+  const WindowDecodeWsLayout L = window_decode_ws_layout(
+      batch_size, num_kv_indices, window_left, num_sink_tokens, kPage,
+      decode_ws_bytes(sh, batch_size, cache->num_kv_heads, cache->head_dim));
+  if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const DecodeWindow win{reinterpret_cast<const int4*>(ws + L.window), kv_indptr, kv_indices};
+  return decode_run(q, q_stride_n, q_stride_h, cache,
+                    reinterpret_cast<const int32_t*>(ws + L.indices),
+                    reinterpret_cast<const int32_t*>(ws + L.indptr), kv_last_page_len, batch_size,
+                    num_qo_heads, sm_scale, ws + L.decode, workspace_bytes - L.decode, out, lse,
+                    stream, app, &win);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pa_window_decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                         const pa_kv_cache* cache, const int32_t* kv_indices,
+                         const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                         int32_t batch_size, int64_t num_kv_indices, int32_t num_qo_heads,
+                         int32_t window_left, int32_t num_sink_tokens, float sm_scale,
+                         void* workspace, size_t workspace_bytes, void* out, float* lse,
+                         void* stream) {
+  return window_decode_run(q, q_stride_n, q_stride_h, cache, kv_indices, kv_indptr,
+                           kv_last_page_len, batch_size, num_kv_indices, num_qo_heads,
+                           window_left, num_sink_tokens, sm_scale, workspace, workspace_bytes,
+                           out, lse, stream, nullptr);
+}
+
+int pa_window_decode_append_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                                const void* append_key, int64_t key_stride_n,
+                                int64_t key_stride_h, const void* append_value,
+                                int64_t value_stride_n, int64_t value_stride_h,
+                                const int32_t* positions, const pa_kv_cache* cache,
+                                const int32_t* kv_indices, const int32_t* kv_indptr,
+                                const int32_t* kv_last_page_len, int32_t batch_size,
+                                int64_t num_kv_indices, int32_t num_qo_heads, int32_t window_left,
+                                int32_t num_sink_tokens, float sm_scale, void* workspace,
+                                size_t workspace_bytes, void* out, float* lse, void* stream) {
+  if (append_key == nullptr || append_value == nullptr || positions == nullptr)
+    return PA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(append_key) || !aligned16(append_value) || key_stride_n % 8 ||
+      key_stride_h % 8 || value_stride_n % 8 || value_stride_h % 8)
+    return PA_ERR_INVALID_ARGUMENT;
+  const DecodeAppend app{append_key, key_stride_n, key_stride_h, append_value,
+                         value_stride_n, value_stride_h, positions, nullptr};
+  return window_decode_run(q, q_stride_n, q_stride_h, cache, kv_indices, kv_indptr,
+                           kv_last_page_len, batch_size, num_kv_indices, num_qo_heads,
+                           window_left, num_sink_tokens, sm_scale, workspace, workspace_bytes,
+                           out, lse, stream, &app);
+}
+
 int pa_merge_states(const void* v, const float* s, int32_t seq_len, int32_t num_states,
                     int32_t num_heads, int32_t head_dim, int32_t dtype, void* v_merged,
                     float* s_merged, void* stream) {
@@ -921,10 +1080,16 @@ size_t pa_prefill_workspace_bytes(int32_t batch_size, int64_t max_total_qo, int3
   return prefill_ws_layout(prefill_max_items(batch_size, max_total_qo, num_kv_heads, span)).total;
 }
 
-int pa_prefill_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
+}  // extern "C"
+
+namespace {
+
+// window_left < 0: full contexts.
+int prefill_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
                     const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
-                    int64_t num_kv_indices, int32_t num_qo_heads, int32_t num_kv_heads,
-                    int32_t head_dim, int32_t page_size, void* workspace, size_t workspace_bytes,
+                 int64_t num_kv_indices, int32_t num_qo_heads, int32_t num_kv_heads,
+                    int32_t head_dim, int32_t page_size, int32_t window_left,
+                    int32_t num_sink_tokens, void* workspace, size_t workspace_bytes,
                     void* stream) {
   if (qo_indptr == nullptr || kv_indptr == nullptr || kv_last_page_len == nullptr ||
       workspace == nullptr)
@@ -942,14 +1107,16 @@ int pa_prefill_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
   // one thread per cost bucket (the plan's scan relies on it)
   prefill_plan_kernel<<<1, kPfCostBuckets, 0, static_cast<cudaStream_t>(stream)>>>(
       qo_indptr, kv_indptr, kv_last_page_len, batch_size, total_qo, num_kv_indices, num_qo_heads,
-      num_kv_heads, head_dim, page_size, span, max_items, static_cast<uint8_t*>(workspace));
+      num_kv_heads, head_dim, page_size, span, max_items, window_left, num_sink_tokens,
+      static_cast<uint8_t*>(workspace));
   return launch_status();
 }
 
-int pa_prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_kv_cache* cache,
+int prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_kv_cache* cache,
                    const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
                    const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
-                   int32_t num_qo_heads, int32_t causal, float sm_scale, void* workspace,
+                   int32_t num_qo_heads, int32_t causal, int32_t window_left,
+                   int32_t num_sink_tokens, float sm_scale, void* workspace,
                    size_t workspace_bytes, void* out, float* lse, void* stream) {
   int st = check_cache(cache);
   if (st != PA_OK) return st;
@@ -1002,13 +1169,62 @@ int pa_prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const 
   p.items = reinterpret_cast<const int4*>(ws + L.items);
   p.sched = reinterpret_cast<int32_t*>(ws + L.hdr + offsetof(PrefillPlanHeader, next_item));
   p.q_rows = nullptr;
+  p.window = window_left;
+  p.sinks = num_sink_tokens;
   const int dev = current_device();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache->dtype == PA_DTYPE_BF16)
-    return D == 64 ? launch_prefill<__nv_bfloat16, 64>(qm, km, vm, om, p, max_items, dev, s)
-                   : launch_prefill<__nv_bfloat16, 128>(qm, km, vm, om, p, max_items, dev, s);
-  return D == 64 ? launch_prefill<__half, 64>(qm, km, vm, om, p, max_items, dev, s)
-                 : launch_prefill<__half, 128>(qm, km, vm, om, p, max_items, dev, s);
+  return window_left >= 0
+             ? launch_prefill_any<true>(cache->dtype, D, qm, km, vm, om, p, max_items, dev, s)
+             : launch_prefill_any<false>(cache->dtype, D, qm, km, vm, om, p, max_items, dev, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pa_prefill_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
+                    const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
+                    int64_t num_kv_indices, int32_t num_qo_heads, int32_t num_kv_heads,
+                    int32_t head_dim, int32_t page_size, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  return prefill_plan(qo_indptr, kv_indptr, kv_last_page_len, batch_size, total_qo,
+                      num_kv_indices, num_qo_heads, num_kv_heads, head_dim, page_size, -1, 0,
+                      workspace, workspace_bytes, stream);
+}
+
+int pa_prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_kv_cache* cache,
+                   const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
+                   const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
+                   int32_t num_qo_heads, int32_t causal, float sm_scale, void* workspace,
+                   size_t workspace_bytes, void* out, float* lse, void* stream) {
+  return prefill_run(q, q_stride_n, q_stride_h, cache, qo_indptr, kv_indices, kv_indptr,
+                     kv_last_page_len, batch_size, total_qo, num_qo_heads, causal, -1, 0, sm_scale,
+                     workspace, workspace_bytes, out, lse, stream);
+}
+
+int pa_window_prefill_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
+                           const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
+                           int64_t num_kv_indices, int32_t num_qo_heads, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t page_size, int32_t window_left,
+                           int32_t num_sink_tokens, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  if (window_left < 0 || num_sink_tokens < 0) return PA_ERR_INVALID_ARGUMENT;
+  return prefill_plan(qo_indptr, kv_indptr, kv_last_page_len, batch_size, total_qo,
+                      num_kv_indices, num_qo_heads, num_kv_heads, head_dim, page_size,
+                      window_left, num_sink_tokens, workspace, workspace_bytes, stream);
+}
+
+int pa_window_prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                          const pa_kv_cache* cache, const int32_t* qo_indptr,
+                          const int32_t* kv_indices, const int32_t* kv_indptr,
+                          const int32_t* kv_last_page_len, int32_t batch_size, int64_t total_qo,
+                          int32_t num_qo_heads, int32_t causal, int32_t window_left,
+                          int32_t num_sink_tokens, float sm_scale, void* workspace,
+                          size_t workspace_bytes, void* out, float* lse, void* stream) {
+  if (window_left < 0 || num_sink_tokens < 0) return PA_ERR_INVALID_ARGUMENT;
+  return prefill_run(q, q_stride_n, q_stride_h, cache, qo_indptr, kv_indices, kv_indptr,
+                     kv_last_page_len, batch_size, total_qo, num_qo_heads, causal, window_left,
+                     num_sink_tokens, sm_scale, workspace, workspace_bytes, out, lse, stream);
 }
 
 }  // extern "C"

@@ -90,12 +90,16 @@ __host__ __device__ inline bool decode_geom(int hkv, int head_dim, DecodeGeom* g
 // --------------------------------------------------------------------- plan
 // One CTA (every thread calls it). Validates the CSR table, cuts the
 // (request, head block, page) stream into runs of Q pages for `num_groups`
-// groups, clears the merge counters.
-__device__ void decode_plan_block(const int32_t* __restrict__ kv_indptr,
+// groups, clears the merge counters. kv_indptr is anything indexable
+// (a pointer, or a view that reads an indptr this CTA has just written);
+// `bad` is an error the caller has found already.
+template <typename Indptr>
+__device__ void decode_plan_block(const Indptr kv_indptr,
                                   const int32_t* __restrict__ last_len, int batch, int hkv,
                                   int hq, int head_dim, int page_size, int64_t num_indices,
                                   int num_groups, int hb, int min_per_group,
-                                  uint8_t* __restrict__ ws) {
+                                  uint8_t* __restrict__ ws, int32_t magic = kDecodeMagic,
+                                  bool bad_table = false) {
   const DecodeWsLayout L = decode_ws_layout(num_groups, batch, hkv, head_dim, hb);
   DecodePlanHeader* hdr = reinterpret_cast<DecodePlanHeader*>(ws + L.hdr);
   int4* unit_start = reinterpret_cast<int4*>(ws + L.unit_start);
@@ -106,7 +110,7 @@ __device__ void decode_plan_block(const int32_t* __restrict__ kv_indptr,
   __shared__ int s_err;
   __shared__ int s_empty;
   if (threadIdx.x == 0) {
-    s_err = 0;
+    s_err = bad_table ? 1 : 0;
     s_empty = 0;
   }
   __syncthreads();
@@ -169,7 +173,7 @@ __device__ void decode_plan_block(const int32_t* __restrict__ kv_indptr,
     hdr->page_size = page_size;
     hdr->num_empty = err ? 0 : s_empty;
     hdr->heads_per_unit = hb;
-    hdr->magic = kDecodeMagic;
+    hdr->magic = magic;
     if (err) set_status(PA_ERR_DEVICE_CHECK);
   }
 }
@@ -312,7 +316,30 @@ __device__ __noinline__ void merge_segments(const float* part_lse, const float* 
     for (int s = 0; s < nseg; ++s) counter[seg[s].b * hkv + seg[s].head] = 0;
 }
 
-template <typename T, int D>
+// Row b's new token of head `head` written into the pool alone: slot `slot`
+// of page `rp` of the caller's table (one 16-byte chunk per lane).
+template <int D>
+__device__ __forceinline__ void append_row_to_pool(const DecodeParams& p, int b, int head, int rp,
+                                                int slot, int lane) {
+  constexpr int CH = D / 8;
+  const int page = __ldg(p.table_indices + __ldg(p.table_indptr + b) + rp);
+  if (page < 0 || page >= p.num_pages) {
+    if (lane == 0) set_status(PA_ERR_DEVICE_CHECK);
+    return;
+  }
+  if (lane < 2 * CH) {
+    const int kv = lane / CH, c = lane - kv * CH;
+    const uint8_t* src = kv ? p.new_v + b * p.new_v_stride_n + head * p.new_v_stride_h
+                            : p.new_k + b * p.new_k_stride_n + head * p.new_k_stride_h;
+    uint8_t* dst = (kv ? p.v_pool : p.k_pool) + page * p.pool_page_stride +
+                   head * p.pool_head_stride + slot * p.pool_token_stride;
+    reinterpret_cast<uint4*>(dst)[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+  }
+}
+
+// kWindow: the table is the compacted one of a sliding-window plan
+// (window.cuh), whose boundary pages hide some of their keys.
+template <typename T, int D, bool kWindow = false>
 __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
     decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                   const DecodeParams p) {
@@ -355,7 +382,7 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
   // for this grid, so the load is in bounds whatever the header holds)
   const int4 st = p.unit_start[grp];
 
-  if (hdr->magic != kDecodeMagic || hdr->num_units != num_groups ||
+  if (hdr->magic != (kWindow ? kWindowDecodeMagic : kDecodeMagic) || hdr->num_units != num_groups ||
       hdr->batch_size != p.batch_size || hdr->num_kv_heads != p.num_kv_heads ||
       hdr->num_qo_heads != p.num_qo_heads || hdr->head_dim != D || hdr->heads_per_unit != HB) {
     if (gw == 0 && lane == 0) set_status(PA_ERR_NOT_PLANNED);
@@ -465,6 +492,7 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
   float o[NT][4];
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   int seg_start = 0, last_len = kPage, head = 0, apos = -1;
+  int hole_lo = 0, hole_hi = 0;  // keys of the segment's stream that the window hides
   const bool row0 = gid < G, row1 = gid + 8 < G;
   // Row of token r of this warp's head inside a panel of the stage.
   const int row_mul = p.heads_inner ? HB : 1;
@@ -504,9 +532,27 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
         // inside the request's pages
         apos = __ldg(p.append_pos + cc.b);
         if (p.append_pos_base != nullptr) apos -= __ldg(p.append_pos_base);
-        if (apos < 0 || apos / kPage >= cc.n) {
+        int pages = cc.n;
+        if constexpr (kWindow) pages += __ldg(&p.window[cc.b].w);
+        if (apos < 0 || apos / kPage >= pages) {
           if (lane == 0) set_status(PA_ERR_DEVICE_CHECK);
           apos = -1;
+        }
+      }
+      if constexpr (kWindow) {
+        const int4 win = __ldg(p.window + cc.b);
+        hole_lo = win.x;
+        hole_hi = win.y;
+        if (apos >= 0 && apos / kPage >= win.z) {
+          const int rp = apos / kPage;
+          if (rp - win.z >= win.w) {
+            apos -= win.w * kPage;  // its place in the compacted stream
+          } else {
+            // behind the window: written (by the one warp that starts the
+            // segment), never read here
+            if (cc.j == 0) append_row_to_pool<D>(p, cc.b, head, rp, apos % kPage, lane);
+            apos = -1;
+          }
         }
       }
     }
@@ -519,6 +565,12 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
     const uint32_t kb = smem_u32(kst);
     const uint32_t vb = kb + PANELS * panel_bytes;
     const int valid = (cc.j == cc.n - 1) ? last_len : kPage;
+    // keys [h0, h1) of this page are hidden by the window
+    int h0 = 0, h1 = 0;
+    if constexpr (kWindow) {
+      h0 = max(hole_lo - cc.j * kPage, 0);
+      h1 = max(min(hole_hi - cc.j * kPage, kPage), h0);
+    }
 
     // ---- decode-step append: this page holds the request's new token
     if (apos >= 0 && cc.j == apos / kPage) {
@@ -568,7 +620,9 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = t * 8 + 2 * tig + (e & 1);
-        s[t][e] = key < valid ? s[t][e] * p.scale_log2 : -INFINITY;
+        bool seen = key < valid;
+        if constexpr (kWindow) seen = seen && (key < h0 || key >= h1);
+        s[t][e] = seen ? s[t][e] * p.scale_log2 : -INFINITY;
       }
       mx0 = fmaxf(mx0, fmaxf(s[t][0], s[t][1]));
       mx1 = fmaxf(mx1, fmaxf(s[t][2], s[t][3]));
@@ -616,6 +670,22 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
       }
       fence_proxy_async();
       __syncwarp();
+    }
+
+    // Hidden keys hold tokens that must not reach O either, whatever they are.
+    if constexpr (kWindow) {
+      if (h0 < h1) {
+        uint8_t* vst = kst + PANELS * panel_bytes;
+        for (int idx = lane; idx < (h1 - h0) * PANELS * 8; idx += 32) {
+          const int r = h0 + idx / (PANELS * 8);
+          const int rem = idx % (PANELS * 8);
+          *reinterpret_cast<uint4*>(vst + (rem >> 3) * panel_bytes +
+                                    (r * row_mul + row_add) * 128 + (rem & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+      }
     }
 
     // ---- O += P V

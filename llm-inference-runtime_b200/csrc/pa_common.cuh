@@ -15,6 +15,7 @@ constexpr int kPage = 16;
 constexpr int kMaxGroup = 16;
 constexpr int32_t kDecodeMagic = 0x50414431;   // "PAD1"
 constexpr int32_t kPrefillMagic = 0x50415031;  // "PAP1"
+constexpr int32_t kWindowDecodeMagic = 0x50415731;  // "PAW1"
 
 // First error recorded by any kernel since the host last read it
 // (pa_device_status). One word per device context.
@@ -108,6 +109,13 @@ struct DecodeParams {
   uint8_t* k_pool;
   uint8_t* v_pool;
   int64_t pool_page_stride, pool_head_stride, pool_token_stride;  // bytes
+  // Sliding window (decode_kernel<T, D, true> only): kv_indptr / kv_indices
+  // above are then the plan's compacted table of visible pages, window[b]
+  // says what is hidden inside it, and table_indptr / table_indices are the
+  // caller's own table (an append may go to a page that is not visible).
+  const int4* window;
+  const int32_t* table_indptr;
+  const int32_t* table_indices;
 };
 
 }  // namespace pa

@@ -33,6 +33,7 @@
 #pragma once
 
 #include "pa_common.cuh"
+#include "window.cuh"
 
 namespace pa {
 
@@ -165,6 +166,9 @@ struct PrefillParams {
   // requests read the same queries while writing their own output rows —
   // the key chunks of a shared prefix (cascade decode).
   const int32_t* q_rows;
+  // Sliding window (prefill_kernel<T, D, true> only): keys before the window
+  // and the first tokens that stay visible (window.cuh).
+  int32_t window, sinks;
 };
 
 // --------------------------------------------------------------------- plan
@@ -179,7 +183,7 @@ __global__ void prefill_plan_kernel(const int32_t* __restrict__ qo_indptr,
                                     const int32_t* __restrict__ last_len, int batch,
                                     int64_t total_qo, int64_t num_indices, int hq, int hkv,
                                     int head_dim, int page_size, int qt, int64_t max_items,
-                                    uint8_t* __restrict__ ws) {
+                                    int window, int sinks, uint8_t* __restrict__ ws) {
   const PrefillWsLayout L = prefill_ws_layout(max_items);
   PrefillPlanHeader* hdr = reinterpret_cast<PrefillPlanHeader*>(ws + L.hdr);
   int4* items = reinterpret_cast<int4*>(ws + L.items);
@@ -197,7 +201,9 @@ __global__ void prefill_plan_kernel(const int32_t* __restrict__ qo_indptr,
     return n > 0 ? (n - 1) * page_size + last_len[b] : 0;
   };
   auto cost_of = [&](int qo_len, int kv_len, int t0) {
-    const int end = min(kv_len, kv_len - qo_len + t0 + qt);
+    int end = min(kv_len, kv_len - qo_len + t0 + qt);
+    if (window >= 0)  // (window < 0: none)
+      end -= window_span(kv_len - qo_len + t0, window, sinks, page_size).shift * page_size;
     const int tiles = end > 0 ? (end + kPfKeys - 1) / kPfKeys : 0;
     return min(tiles, kPfCostBuckets - 1);
   };
@@ -301,12 +307,19 @@ __global__ void prefill_plan_kernel(const int32_t* __restrict__ qo_indptr,
 // One item's geometry, as every warp of the CTA needs it.
 struct PfItem {
   int b, h, t0, qo_start, qo_len, q_row0, page0, npages, kv_len, ntiles;  // ntiles < 0: stop
+  // sliding window: npages counts the item's visible pages; page v of them is
+  // table page v + (v < sink_pages ? 0 : shift), and the keys [hole_lo,
+  // hole_hi) of that stream are hidden from every query of the item
+  int hole_lo, hole_hi, sink_pages, shift;
 };
+static_assert(sizeof(PfItem) <= 64, "one slot of the work-item ring");
 
+template <bool kWindow>
 __device__ __forceinline__ PfItem pf_item(const PrefillParams& p, int idx) {
   PfItem w;
+  w.hole_lo = w.hole_hi = w.sink_pages = w.shift = 0;
   if (idx < 0) {
-    w = PfItem{0, 0, 0, 0, 0, 0, 0, 0, 0, -1};
+    w = PfItem{0, 0, 0, 0, 0, 0, 0, 0, 0, -1, 0, 0, 0, 0};
     return w;
   }
   const int4 it = p.items[idx];
@@ -321,12 +334,23 @@ __device__ __forceinline__ PfItem pf_item(const PrefillParams& p, int idx) {
   w.kv_len = w.npages > 0 ? (w.npages - 1) * kPage + __ldg(p.kv_last_page_len + w.b) : 0;
   // keys this item can see: up to its last query's position (causal) or all
   const int q_hi = min(w.t0 + 2 * p.qt, w.qo_len);
-  const int kv_end = p.causal ? min(w.kv_len, w.kv_len - w.qo_len + q_hi) : w.kv_len;
+  int kv_end = p.causal ? min(w.kv_len, w.kv_len - w.qo_len + q_hi) : w.kv_len;
+  if constexpr (kWindow) {
+    const WindowSpan s = window_span(w.kv_len - w.qo_len + w.t0, p.window, p.sinks, kPage);
+    w.hole_lo = s.hole_lo;
+    w.hole_hi = s.hole_hi;
+    w.sink_pages = s.sink_pages;
+    w.shift = s.shift;
+    w.npages -= s.shift;
+    kv_end -= s.shift * kPage;
+  }
   w.ntiles = kv_end > 0 ? (kv_end + kPfKeys - 1) / kPfKeys : 0;
   return w;
 }
 
-template <typename T, int D>
+// kWindow: sliding window with sinks. An item's keys are then the stream of
+// its visible pages (window.cuh); everything below counts in that stream.
+template <typename T, int D, bool kWindow = false>
 __global__ void __launch_bounds__(kPfThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap omap,
@@ -414,7 +438,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     PfItem w;
     if (!mbar_wait_warp(&item_full[it % 3], (it / 3) & 1)) {
       failed = true;
-      w = PfItem{0, 0, 0, 0, 0, 0, 0, 0, 0, -1};
+      w = PfItem{0, 0, 0, 0, 0, 0, 0, 0, 0, -1, 0, 0, 0, 0};
     } else {
       w = slots[it % 3];
     }
@@ -448,7 +472,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       __syncwarp();
     };
-    PfItem w = pf_item(p, claim());
+    PfItem w = pf_item<kWindow>(p, claim());
     publish(0, w);
     uint32_t kt = 0;  // K / V tiles loaded so far: ring position
     int qc = 0;       // items whose Q tiles were loaded
@@ -481,7 +505,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const int nxt = claim();
       if (it >= 2 && !mbar_wait_warp(&item_empty[(it + 1) % 3], ((it - 2) / 3) & 1))
         failed = true;
-      const PfItem wn = pf_item(p, failed ? -1 : nxt);
+      const PfItem wn = pf_item<kWindow>(p, failed ? -1 : nxt);
       publish((it + 1) % 3, wn);
       const int c1 = p.heads_inner ? w.h : 0, c2 = p.heads_inner ? 0 : w.h;
       if (w.ntiles > 0) {
@@ -502,7 +526,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const int np = min(8, w.npages - 8 * j);
         int page = 0;
         if (lane < np) {
-          page = __ldg(p.kv_indices + w.page0 + 8 * j + lane);
+          int v = 8 * j + lane;
+          if constexpr (kWindow) v += v < w.sink_pages ? 0 : w.shift;
+          page = __ldg(p.kv_indices + w.page0 + v);
           if (static_cast<unsigned>(page) >= static_cast<unsigned long long>(p.num_pages)) {
             set_status(PA_ERR_DEVICE_CHECK);
             page = 0;
@@ -707,12 +733,23 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     uint32_t kt = 0;  // running tile count = running step count
     for (int it = 0;; ++it) {
     int ntiles, kv_len, lim;
+    int hole_lo = 0, hole_hi = 0;    // hidden from this row
+    int ihole_lo = 0, ihole_hi = 0;  // hidden from every row of the item
     {
       const PfItem w = wait_item(it);
       ntiles = w.ntiles;
       kv_len = w.kv_len;
       const int qpos = kv_len - w.qo_len + w.t0 + qi;
       lim = p.causal ? min(qpos + 1, kv_len) : kv_len;
+      if constexpr (kWindow) {
+        const int skip = w.shift * kPage;
+        kv_len -= skip;
+        lim -= skip;
+        hole_lo = p.sinks;
+        hole_hi = max(qpos - p.window, 0) - skip;
+        ihole_lo = w.hole_lo;
+        ihole_hi = w.hole_hi;
+      }
     }
     if (ntiles < 0) {
       done_item(it);
@@ -735,7 +772,20 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       for (int c = 0; c < kPfKeys / 32; ++c) tmem_ld32(tS + c * 32, s + c * 32);
       tmem_wait_ld();
       const int key0 = j * kPfKeys;
-      if (!__all_sync(0xffffffffu, key0 + kPfKeys <= lim)) {
+      if constexpr (kWindow) {
+        // hidden: columns >= lim - key0, and columns [a, b)
+        const int a = hole_lo - key0, b = hole_hi - key0, e = lim - key0;
+        if (!__all_sync(0xffffffffu, e >= kPfKeys)) {
+#pragma unroll
+          for (int c = 0; c < kPfKeys; ++c)
+            if (c >= e) s[c] = -INFINITY;
+        }
+        if (!__all_sync(0xffffffffu, a >= kPfKeys || b <= 0 || a >= b)) {
+#pragma unroll
+          for (int c = 0; c < kPfKeys; ++c)
+            if (c >= a && c < b) s[c] = -INFINITY;
+        }
+      } else if (!__all_sync(0xffffffffu, key0 + kPfKeys <= lim)) {
 #pragma unroll
         for (int c = 0; c < kPfKeys; ++c)
           if (key0 + c >= lim) s[c] = -INFINITY;
@@ -791,13 +841,21 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       // The last tile may hold keys past kv_len (stale slots, pages never
       // loaded): tile 0's warpgroup zeroes those V rows before its PV, which
       // precedes tile 1's PV on the tensor pipe.
-      if (t == 0 && j == ntiles - 1 && key0 + kPfKeys > kv_len) {
+      bool clear = j == ntiles - 1 && key0 + kPfKeys > kv_len;
+      // the same for keys that the window hides from the whole item: their
+      // tokens must not reach O, whatever they are
+      if constexpr (kWindow)
+        clear = clear || (ihole_lo < ihole_hi && ihole_lo < key0 + kPfKeys && ihole_hi > key0);
+      if (t == 0 && clear) {
         const int st = g % S;
         if (!mbar_wait_warp(&v_full[st], (g / S) & 1)) {
           failed = true;
           break;
         }
-        if (key0 + r >= kv_len) {
+        bool drop = key0 + r >= kv_len;
+        if constexpr (kWindow)
+          drop = drop || (key0 + r >= ihole_lo && key0 + r < ihole_hi);
+        if (drop) {
 #pragma unroll
           for (int pn = 0; pn < C::kPanels; ++pn)
 #pragma unroll

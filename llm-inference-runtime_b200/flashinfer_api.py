@@ -13,6 +13,9 @@ so ``models/llama.py`` works with ``import flashinfer`` pointed here:
 * ``BatchDecodeWithPagedKVCacheWrapper`` plan/begin_forward/run/forward
   (llama.py:62-67, 138, 236)
 * ``merge_state`` / ``merge_states`` / ``get_seq_lens`` (split-KV helpers)
+* ``BatchDecodeWithSlidingWindowWrapper`` / ``BatchPrefillWithSlidingWindowWrapper``
+  (this package's: the two wrappers above over the last keys of each context
+  and its first tokens)
 * ``MultiLevelCascadeAttentionWrapper`` (two levels: a prefix every request
   shares, then each request's own pages) for radix-shared decode batches
 
@@ -315,12 +318,16 @@ class BatchDecodeWithPagedKVCacheWrapper:
         self._q_dtype = _as_dtype(data_type) or _as_dtype(q_data_type)
         self._kv_dtype = _as_dtype(kv_data_type) or self._q_dtype
         self._sm_scale = sm_scale
-        _lib.check(_lib.load().pa_decode_plan(
-            _p(self._indptr), _p(self._last), self._batch, self._indices.numel(), num_qo_heads,
-            num_kv_heads, head_dim, page_size, _p(self._ws), self._ws.numel() *
-            self._ws.element_size(), _stream()), "BatchDecodeWithPagedKVCacheWrapper.plan")
-        _after("BatchDecodeWithPagedKVCacheWrapper.plan")
+        what = type(self).__name__ + ".plan"
+        _lib.check(self._plan_call(), what)
+        _after(what)
         self._planned = True
+
+    def _plan_call(self) -> int:
+        return _lib.load().pa_decode_plan(
+            _p(self._indptr), _p(self._last), self._batch, self._indices.numel(), self._hq,
+            self._hkv, self._d, self._p, _p(self._ws),
+            self._ws.numel() * self._ws.element_size(), _stream())
 
     begin_forward = plan
 
@@ -375,24 +382,23 @@ class BatchDecodeWithPagedKVCacheWrapper:
             lse = torch.empty((self._batch, self._hq), dtype=torch.float32, device=q.device)
         scale = self._sm_scale if self._sm_scale is not None else 1.0 / math.sqrt(self._d)
         scale *= _check_scales(q_scale, k_scale, v_scale)
+        what = type(self).__name__ + (".run" if append is None else ".run_with_append")
+        _lib.check(self._run_call(q, qsn, qsh, desc, append, float(scale), out, lse), what)
+        _after(what)
+        return (out, lse) if return_lse else out
+
+    def _run_call(self, q, qsn, qsh, desc, append, scale, out, lse) -> int:
         ws_bytes = self._ws.numel() * self._ws.element_size()
         if append is None:
-            _lib.check(_lib.load().pa_decode_run(
+            return _lib.load().pa_decode_run(
                 _p(q), qsn, qsh, ctypes.byref(desc), _p(self._indices), _p(self._indptr),
-                _p(self._last), self._batch, self._hq, float(scale), _p(self._ws), ws_bytes,
-                _p(out), _p(lse), _stream()), "BatchDecodeWithPagedKVCacheWrapper.run")
-            _after("BatchDecodeWithPagedKVCacheWrapper.run")
-        else:
-            k, v, pos = append
-            ksn, ksh = k.stride(0), k.stride(1)
-            vsn, vsh = v.stride(0), v.stride(1)
-            _lib.check(_lib.load().pa_decode_append_run(
-                _p(q), qsn, qsh, _p(k), ksn, ksh, _p(v), vsn, vsh, _p(pos), ctypes.byref(desc),
-                _p(self._indices), _p(self._indptr), _p(self._last), self._batch, self._hq,
-                float(scale), _p(self._ws), ws_bytes, _p(out), _p(lse), _stream()),
-                "BatchDecodeWithPagedKVCacheWrapper.run_with_append")
-            _after("BatchDecodeWithPagedKVCacheWrapper.run_with_append")
-        return (out, lse) if return_lse else out
+                _p(self._last), self._batch, self._hq, scale, _p(self._ws), ws_bytes,
+                _p(out), _p(lse), _stream())
+        k, v, pos = append
+        return _lib.load().pa_decode_append_run(
+            _p(q), qsn, qsh, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
+            _p(pos), ctypes.byref(desc), _p(self._indices), _p(self._indptr), _p(self._last),
+            self._batch, self._hq, scale, _p(self._ws), ws_bytes, _p(out), _p(lse), _stream())
 
     def forward(self, q: torch.Tensor, paged_kv_cache, pos_encoding_mode: str = "NONE",
                 q_scale=None, k_scale=None, v_scale=None, window_left: int = -1,
@@ -481,14 +487,17 @@ class BatchPrefillWithPagedKVCacheWrapper:
         pass
 
     def _device_plan(self, total_qo: int) -> None:
-        _lib.check(_lib.load().pa_prefill_plan(
-            _p(self._qo_indptr), _p(self._indptr), _p(self._last), self._batch, total_qo,
-            self._indices.numel(), self._hq, self._hkv, self._d, self._p, _p(self._ws),
-            self._ws.numel() * self._ws.element_size(), _stream()),
-            "BatchPrefillWithPagedKVCacheWrapper.plan")
-        _after("BatchPrefillWithPagedKVCacheWrapper.plan")
+        what = type(self).__name__ + ".plan"
+        _lib.check(self._plan_call(total_qo), what)
+        _after(what)
         self._plan_total = total_qo
         self._needs_device_plan = False
+
+    def _plan_call(self, total_qo: int) -> int:
+        return _lib.load().pa_prefill_plan(
+            _p(self._qo_indptr), _p(self._indptr), _p(self._last), self._batch, total_qo,
+            self._indices.numel(), self._hq, self._hkv, self._d, self._p, _p(self._ws),
+            self._ws.numel() * self._ws.element_size(), _stream())
 
     def run(self, q: torch.Tensor, paged_kv_cache, *args, q_scale=None, k_scale=None,
             v_scale=None, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
@@ -514,14 +523,17 @@ class BatchPrefillWithPagedKVCacheWrapper:
             lse = torch.empty((total_qo, self._hq), dtype=torch.float32, device=q.device)
         scale = self._sm_scale if self._sm_scale is not None else 1.0 / math.sqrt(self._d)
         scale *= _check_scales(q_scale, k_scale, v_scale)
-        _lib.check(_lib.load().pa_prefill_run(
+        what = type(self).__name__ + ".run"
+        _lib.check(self._run_call(q, qsn, qsh, desc, total_qo, float(scale), out, lse), what)
+        _after(what)
+        return (out, lse) if return_lse else out
+
+    def _run_call(self, q, qsn, qsh, desc, total_qo, scale, out, lse) -> int:
+        return _lib.load().pa_prefill_run(
             _p(q), qsn, qsh, ctypes.byref(desc), _p(self._qo_indptr), _p(self._indices),
             _p(self._indptr), _p(self._last), self._batch, total_qo, self._hq,
-            int(self._causal), float(scale), _p(self._ws),
-            self._ws.numel() * self._ws.element_size(), _p(out), _p(lse), _stream()),
-            "BatchPrefillWithPagedKVCacheWrapper.run")
-        _after("BatchPrefillWithPagedKVCacheWrapper.run")
-        return (out, lse) if return_lse else out
+            int(self._causal), scale, _p(self._ws),
+            self._ws.numel() * self._ws.element_size(), _p(out), _p(lse), _stream())
 
     def forward(self, q: torch.Tensor, paged_kv_cache, causal: bool = False,
                 pos_encoding_mode: str = "NONE", use_fp16_qk_reduction: bool = False,
@@ -544,6 +556,78 @@ class BatchPrefillWithPagedKVCacheWrapper:
         if sm_scale is not None:
             self._sm_scale = sm_scale
         return self.run(q, paged_kv_cache, k_scale=k_scale, v_scale=v_scale, return_lse=True)
+
+
+def _check_window(window_left, num_sink_tokens) -> Tuple[int, int]:
+    window_left, num_sink_tokens = int(window_left), int(num_sink_tokens)
+    if not 0 <= window_left < 2 ** 31:
+        raise ValueError("window_left must be in [0, 2**31)")
+    if not 0 <= num_sink_tokens < 2 ** 31:
+        raise ValueError("num_sink_tokens must be in [0, 2**31)")
+    return window_left, num_sink_tokens
+
+
+class BatchDecodeWithSlidingWindowWrapper(BatchDecodeWithPagedKVCacheWrapper):
+    """Batched decode in which request b's query, at position ``kv_len - 1``,
+    sees key j iff ``kv_len - 1 - j <= window_left`` or ``j < num_sink_tokens``
+    (FlashInfer's ``window_left`` plus first tokens that stay visible).
+
+    Constructed with the window, used like
+    :class:`BatchDecodeWithPagedKVCacheWrapper`. Pages without a visible key
+    are not read, and neither are their entries of ``indices``, which may be
+    -1 (``pages.evict_window_pages`` gives such pages back). ``plan`` copies
+    the visible page ids into the workspace, so the page table is planned
+    anew for every step, as the reference does."""
+
+    def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD", *,
+                 window_left: int, num_sink_tokens: int = 0, **kwargs) -> None:
+        super().__init__(float_workspace_buffer, kv_layout, **kwargs)
+        self._window, self._sinks = _check_window(window_left, num_sink_tokens)
+
+    def _plan_call(self) -> int:
+        return _lib.load().pa_window_decode_plan(
+            _p(self._indptr), _p(self._indices), _p(self._last), self._batch,
+            self._indices.numel(), self._hq, self._hkv, self._d, self._p, self._window,
+            self._sinks, _p(self._ws), self._ws.numel() * self._ws.element_size(), _stream())
+
+    def _run_call(self, q, qsn, qsh, desc, append, scale, out, lse) -> int:
+        table = (ctypes.byref(desc), _p(self._indices), _p(self._indptr), _p(self._last),
+                 self._batch, self._indices.numel(), self._hq, self._window, self._sinks, scale,
+                 _p(self._ws), self._ws.numel() * self._ws.element_size(), _p(out), _p(lse),
+                 _stream())
+        if append is None:
+            return _lib.load().pa_window_decode_run(_p(q), qsn, qsh, *table)
+        k, v, pos = append
+        return _lib.load().pa_window_decode_append_run(
+            _p(q), qsn, qsh, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
+            _p(pos), *table)
+
+
+class BatchPrefillWithSlidingWindowWrapper(BatchPrefillWithPagedKVCacheWrapper):
+    """Ragged (chunked) prefill in which a query at position p sees key j iff
+    ``p - j <= window_left`` or ``j < num_sink_tokens``, and ``j <= p`` when
+    causal. Constructed with the window, used like
+    :class:`BatchPrefillWithPagedKVCacheWrapper`; pages that no query of a
+    request sees are not read (see
+    :class:`BatchDecodeWithSlidingWindowWrapper`)."""
+
+    def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD", *,
+                 window_left: int, num_sink_tokens: int = 0, **kwargs) -> None:
+        super().__init__(float_workspace_buffer, kv_layout, **kwargs)
+        self._window, self._sinks = _check_window(window_left, num_sink_tokens)
+
+    def _plan_call(self, total_qo: int) -> int:
+        return _lib.load().pa_window_prefill_plan(
+            _p(self._qo_indptr), _p(self._indptr), _p(self._last), self._batch, total_qo,
+            self._indices.numel(), self._hq, self._hkv, self._d, self._p, self._window,
+            self._sinks, _p(self._ws), self._ws.numel() * self._ws.element_size(), _stream())
+
+    def _run_call(self, q, qsn, qsh, desc, total_qo, scale, out, lse) -> int:
+        return _lib.load().pa_window_prefill_run(
+            _p(q), qsn, qsh, ctypes.byref(desc), _p(self._qo_indptr), _p(self._indices),
+            _p(self._indptr), _p(self._last), self._batch, total_qo, self._hq,
+            int(self._causal), self._window, self._sinks, scale, _p(self._ws),
+            self._ws.numel() * self._ws.element_size(), _p(out), _p(lse), _stream())
 
 
 class MultiLevelCascadeAttentionWrapper:
