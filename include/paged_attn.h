@@ -48,7 +48,8 @@ enum pa_status {
   PA_ERR_NOT_PLANNED = 7         /* run called on a workspace without a matching plan */
 };
 
-enum pa_dtype { PA_DTYPE_F16 = 0, PA_DTYPE_BF16 = 1 };
+/* PA_DTYPE_F32: logits of pa_beam_select only. */
+enum pa_dtype { PA_DTYPE_F16 = 0, PA_DTYPE_BF16 = 1, PA_DTYPE_F32 = 2 };
 
 enum pa_kv_layout { PA_LAYOUT_NHD = 0, PA_LAYOUT_HND = 1 };
 
@@ -71,8 +72,10 @@ const char* pa_status_string(int status);
 
 /* ABI version this header describes (major * 100 + minor). 101: the append,
  * RoPE + append, fused QKV and cascade-plan calls take the number of page ids
- * (num_kv_indices) after kv_indptr. 102: the pa_window_* calls. A caller built
- * against another version must refuse the library (the Python binding does). */
+ * (num_kv_indices) after kv_indptr. 102: the pa_window_* calls,
+ * pa_release_pages, pa_fork_sequences, pa_compact_pages, pa_beam_select. A
+ * caller built against another version must refuse the library (the Python
+ * binding does). */
 #define PA_ABI_VERSION 102
 
 /* ABI version of this library (major * 100 + minor); equals PA_ABI_VERSION
@@ -192,6 +195,84 @@ int pa_fork_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
                   int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
                   const int32_t* src_pages, const int32_t* dst_pages, int32_t num_pairs,
                   void* stream);
+
+/* Page bookkeeping on the device: what the reference's BlockAllocator
+ * (src/engine/memory/allocator.py) keeps on the host as a reference count per
+ * page and a block table per sequence, as int32 device arrays.
+ *   ref_counts[num_pages]   holders of a page (tables, a prefix cache); 0 = free
+ *   block_tables[rows][max_blocks], rows block_table_stride elements apart:
+ *     page of tokens [j * page_size, (j + 1) * page_size) of a row, -1 = given back
+ *   seq_lens[rows]          tokens a row holds; its entries j < ceil(len / page_size)
+ * Counting errors that only the device sees (a page id outside the pool, a
+ * count that would fall below zero, no free page left) are added to counts[2]
+ * and recorded as PA_ERR_DEVICE_CHECK; sound rows are processed all the same.
+ *
+ * pa_release_pages, window_left >= 0: entries of pages that lie wholly behind
+ * the window of the row's last token, that is
+ *   ceil(num_sink_tokens / page_size) <= j < floor((len - 1 - window_left) / page_size),
+ * lose one reference and become -1 (pa_window_* calls do not read them).
+ * window_left < 0: every entry of the row does, and its length becomes 0
+ * (a sequence that has ended). counts (device int32[3]) receives {entries
+ * given back, pages whose count reached 0, errors}. */
+int pa_release_pages(int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                     int32_t* seq_lens, int32_t batch_size, int32_t page_size,
+                     int32_t window_left, int32_t num_sink_tokens, int32_t* ref_counts,
+                     int64_t num_pages, int32_t* counts, void* stream);
+
+/* Row r of the new tables continues row parents[r] of the old ones (beam
+ * search's reordering, parallel samples of one prompt): out_seq_lens[r] =
+ * seq_lens[parents[r]], full pages are shared, and the page of the next token,
+ * entry len / page_size, is the row's own: a free page when len is a multiple
+ * of page_size; otherwise the parent's unfinished page, which its first
+ * continuing row keeps if no other holder is left, while every other one gets
+ * a free page and a copy of it in all layers. Rows nobody continues lose
+ * their references. Free pages (count 0 once all references are counted) are
+ * taken lowest number first, by ascending r. Entries past the row's are -1.
+ * counts receives {pages copied, pages taken, rows left without a page (their
+ * entry is -1)}. pool, strides and page_bytes as for pa_fork_pages;
+ * out_block_tables must not be block_tables; workspace: 3 * num_sequences
+ * int32. */
+int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                      int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                      const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                      const int32_t* seq_lens, const int32_t* parents, int32_t num_sequences,
+                      int32_t page_size, int32_t* ref_counts, int32_t* out_block_tables,
+                      int64_t out_stride, int32_t* out_seq_lens, int32_t* counts,
+                      int32_t* workspace, void* stream);
+
+/* Moves the live pages (count > 0) to the front of the pool: with n of them,
+ * the k-th live page at or past n goes to the k-th free page before n, in all
+ * layers. ref_counts follow, the tables' entries too; remap[num_pages]
+ * receives each live page's new number, -1 for free ones (for holders outside
+ * the tables). counts receives {live pages, pages moved, errors}. workspace:
+ * num_pages + 2 int32. */
+int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                     int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                     int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                     const int32_t* seq_lens, int32_t batch_size, int32_t page_size,
+                     int32_t* ref_counts, int32_t* remap, int32_t* counts, int32_t* workspace,
+                     void* stream);
+
+/* Beam search's selection. logits [batch, num_beams, vocab_size] (strides in
+ * elements, last dim contiguous, any alignment; F16 / BF16 / F32), scores
+ * [batch, num_beams] float accumulated log probabilities. A continuation of
+ * beam w with token v scores
+ *   scores[b, w] + (logits[b, w, v] - lse),  lse = log sum_v exp(logits[b, w, v])
+ * (lse rounded to fp32, the sum of the three ordered in fp64). The
+ * num_candidates <= 32 best of a request (num_beams <= 256, vocab_size <=
+ * 2^24), best first; equal scores by the lowest beam, inside a beam by the
+ * larger logit, then the lowest token: out_scores (fp32), out_parents
+ * (b * num_beams + w, a row of pa_fork_sequences), out_tokens, each
+ * [batch, num_candidates].
+ * A NaN logit counts as -inf, +inf as the largest finite value; beams whose
+ * score is -inf or NaN and rows without a finite logit score -inf. */
+size_t pa_beam_select_workspace_bytes(int32_t batch_size, int32_t num_beams, int32_t vocab_size,
+                                      int32_t num_candidates, int32_t dtype);
+int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_stride_w,
+                   const float* scores, int64_t scores_stride_b, int32_t batch_size,
+                   int32_t num_beams, int32_t vocab_size, int32_t num_candidates, int32_t dtype,
+                   float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 /* Replaces the per-layer prologue of the reference's patched attention
  * (src/models/llama.py:163-210): qkv = x W^T with W the fused [q; k; v]

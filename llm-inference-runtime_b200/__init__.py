@@ -16,16 +16,19 @@ Modules:
                  merge_state(s)
   llama          init_flashinfer_state / plan_* / patched attention forward
   tables         device-side step tables (decode / prefill-chunk CSR build)
+  pages          reference counts and block tables on the device: giving pages
+                 back, forking sequences, compaction
+  beam           beam search: selection over beams and vocabulary, the step
   workloads      seeded synthetic configurations (benchmarks and tests)
 """
 
 from . import _lib, build  # noqa: F401
 
-__all__ = ["_lib", "build", "flashinfer_api", "llama", "tables", "workloads"]
+__all__ = ["_lib", "beam", "build", "flashinfer_api", "llama", "pages", "tables", "workloads"]
 
 
 def __getattr__(name):
-    if name in ("flashinfer_api", "llama", "workloads"):
+    if name in ("beam", "flashinfer_api", "llama", "pages", "workloads"):
         import importlib
         return importlib.import_module(f"{__name__}.{name}")
     raise AttributeError(name)

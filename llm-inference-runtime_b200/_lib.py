@@ -28,6 +28,7 @@ PA_ERR_NOT_PLANNED = 7
 
 PA_DTYPE_F16 = 0
 PA_DTYPE_BF16 = 1
+PA_DTYPE_F32 = 2  # logits of pa_beam_select only
 
 PA_NOALLOC_SCRATCH_BYTES = 24 * 1024 * 1024
 
@@ -93,6 +94,28 @@ SIGNATURES = {
         c_int32,
         [c_void_p, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32,
          c_void_p],
+    ),
+    "pa_release_pages": (
+        c_int32,
+        [c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
+         c_int64, c_void_p, c_void_p],
+    ),
+    "pa_fork_sequences": (
+        c_int32,
+        [c_void_p, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
+         c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+         c_void_p, c_void_p],
+    ),
+    "pa_compact_pages": (
+        c_int32,
+        [c_void_p, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
+         c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "pa_beam_select_workspace_bytes": (c_size_t, [c_int32] * 5),
+    "pa_beam_select": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
+         c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
     "pa_qkv_rope_append": (
         c_int32,

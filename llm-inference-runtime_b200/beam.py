@@ -1,0 +1,95 @@
+"""Beam search over the paged cache: selection and the reordering of states.
+
+The reference decodes greedily or by sampling, one sequence per request
+(src/engine/runtime/step_executor.py:204-260). These calls add what a step of
+beam search needs between the model's logits and the next forward: the best
+continuations of each request's beams, and the cache following them
+(``pages.fork_sequences``), on the device without a synchronisation.
+"""
+
+from __future__ import annotations
+
+from typing import Dict, Tuple
+
+import torch
+
+from . import _lib, pages
+from .flashinfer_api import _after
+
+_DTYPES = {torch.float16: _lib.PA_DTYPE_F16, torch.bfloat16: _lib.PA_DTYPE_BF16,
+           torch.float32: _lib.PA_DTYPE_F32}
+MAX_CANDIDATES = 32
+MAX_BEAMS = 256
+MAX_VOCAB = 2 ** 24
+
+
+def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int
+                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``num_candidates`` best continuations of each request.
+
+    logits [batch, beams, vocab] (float16 / bfloat16 / float32, last dim
+    contiguous), scores [batch, beams] float32: accumulated log probabilities
+    (-inf: a beam that does not continue, as all but the first of a request
+    have before the first step). A continuation scores ``scores[b, w] +
+    log_softmax(logits[b, w])[v]``. Returns (scores, parents, tokens), each
+    [batch, num_candidates], best first; equal scores by the lowest beam,
+    inside a beam by the larger logit, then the lowest token. parents are
+    rows ``b * beams + w``, as ``pages.fork_sequences`` takes them. A NaN
+    logit counts as -inf."""
+    if logits.dim() != 3 or scores.dim() != 2 or logits.shape[:2] != scores.shape:
+        raise ValueError("logits must be [batch, beams, vocab] and scores [batch, beams]")
+    if logits.dtype not in _DTYPES:
+        raise NotImplementedError(f"logits of {logits.dtype} are not supported")
+    if scores.dtype != torch.float32:
+        raise TypeError("scores must be float32")
+    if not logits.is_cuda or scores.device != logits.device:
+        raise ValueError("logits and scores must be on one GPU")
+    batch, beams, vocab = logits.shape
+    n = int(num_candidates)
+    if beams == 0 or vocab == 0 or not 1 <= n <= beams * vocab:
+        raise ValueError("num_candidates must be in [1, beams * vocab]")
+    if n > MAX_CANDIDATES or beams > MAX_BEAMS or vocab > MAX_VOCAB:
+        raise NotImplementedError(f"at most {MAX_CANDIDATES} candidates of {MAX_BEAMS} beams and "
+                                  f"{MAX_VOCAB} tokens")
+    if vocab > 1 and logits.stride(2) != 1:
+        raise ValueError("the vocabulary dimension of logits must be contiguous")
+    if scores.size(1) > 1 and scores.stride(1) != 1:
+        scores = scores.contiguous()
+    device = logits.device
+    dtype = _DTYPES[logits.dtype]
+    out = torch.empty((3, batch, n), dtype=torch.int32, device=device)
+    best, parents, tokens = out[0].view(torch.float32), out[1], out[2]
+    if batch == 0:
+        return best, parents, tokens
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        size = lib.pa_beam_select_workspace_bytes(batch, beams, vocab, n, dtype)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        _lib.check(lib.pa_beam_select(
+            logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(),
+            scores.stride(0), batch, beams, vocab, n, dtype, best.data_ptr(), parents.data_ptr(),
+            tokens.data_ptr(), ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream),
+            "beam_search_select")
+        _after("beam_search_select")
+    return best, parents, tokens
+
+
+def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.Tensor,
+                     block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                     ref_counts: torch.Tensor) -> Dict[str, torch.Tensor]:
+    """One step of beam search: each request's beams are replaced by its
+    ``beams`` best continuations and their cache follows.
+
+    Row ``b * beams + w`` of ``block_tables`` / ``seq_lens`` is beam w of
+    request b. Returns scores, parents and tokens [batch, beams] and the new
+    block_tables, seq_lens and counts (``pages.fork_sequences``): every beam
+    owns the page that its token, to be fed to the model next, is appended
+    to, at position seq_lens[r]."""
+    batch, beams = scores.shape
+    if seq_lens.numel() != batch * beams:
+        raise ValueError("block_tables must hold one row per beam of each request")
+    best, parents, tokens = beam_search_select(logits, scores, beams)
+    tables, lens, counts = pages.fork_sequences(kv_pool, block_tables, seq_lens,
+                                                parents.view(-1), ref_counts)
+    return {"scores": best, "parents": parents, "tokens": tokens, "block_tables": tables,
+            "seq_lens": lens, "counts": counts}

@@ -19,6 +19,8 @@
 #include "qkv.cuh"
 #include "cascade.cuh"
 #include "window.cuh"
+#include "pages.cuh"
+#include "beam.cuh"
 
 namespace {
 
@@ -597,6 +599,295 @@ int pa_fork_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
   const int blocks = static_cast<int>(std::min<int64_t>((work + 255) / 256, max_blocks));
   fork_pages_kernel<<<blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
   return launch_status();
+}
+
+}  // extern "C"
+
+namespace {
+
+// Copies src[i] -> dst[i], i < *count (device), in every layer. `most` bounds
+// the pairs (it sizes the grid).
+int launch_copy_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                      int64_t page_stride_bytes, int64_t page_bytes, const int32_t* src,
+                      const int32_t* dst, const int32_t* count, int64_t most,
+                      cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  const int dev = current_device();
+  if (allow_smem(copy_pages_kernel, kCopySmem, &done, dev) != cudaSuccess) return PA_ERR_CUDA;
+  CopyParams c;
+  c.pool = static_cast<uint8_t*>(pool);
+  c.layer_stride = layer_stride_bytes;
+  c.page_stride = page_stride_bytes;
+  c.page_bytes = page_bytes;
+  c.num_layers = num_layers;
+  c.src = src;
+  c.dst = dst;
+  c.count = count;
+  const int64_t units = most * num_layers * ((page_bytes + kCopySlice - 1) / kCopySlice);
+  const int64_t sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min(units, sms)));
+  return launch_chain(copy_pages_kernel, dim3(grid), dim3(32), kCopySmem, stream, c);
+}
+
+// The pool arguments of the calls that move pages.
+int check_pool(const void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+               int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages) {
+  if (num_layers < 0 || num_pages <= 0 || num_pages > 0x7fffffffLL || page_bytes < 0)
+    return PA_ERR_INVALID_ARGUMENT;
+  if (num_layers == 0 || page_bytes == 0) return PA_OK;
+  if (pool == nullptr || !aligned16(pool) || page_bytes % 16 || page_stride_bytes % 16 ||
+      layer_stride_bytes % 16 || page_bytes > page_stride_bytes)
+    return PA_ERR_INVALID_ARGUMENT;
+  return PA_OK;
+}
+
+int check_tables(const void* tables, int64_t stride, int32_t width, int32_t rows,
+                 int32_t page_size) {
+  if (rows < 0 || width < 0 || stride < width || page_size <= 0) return PA_ERR_INVALID_ARGUMENT;
+  if (rows > 0 && width > 0 && tables == nullptr) return PA_ERR_INVALID_ARGUMENT;
+  return PA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pa_release_pages(int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                     int32_t* seq_lens, int32_t batch_size, int32_t page_size,
+                     int32_t window_left, int32_t num_sink_tokens, int32_t* ref_counts,
+                     int64_t num_pages, int32_t* counts, void* stream) {
+  const int st = check_tables(block_tables, block_table_stride, max_blocks, batch_size, page_size);
+  if (st != PA_OK) return st;
+  if (counts == nullptr || num_pages <= 0 || ref_counts == nullptr || num_sink_tokens < 0 ||
+      (batch_size > 0 && seq_lens == nullptr))
+    return PA_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cudaMemsetAsync(counts, 0, 3 * sizeof(int32_t), s) != cudaSuccess) return PA_ERR_CUDA;
+  if (batch_size == 0) return PA_OK;
+  ReleaseParams p;
+  p.tables = block_tables;
+  p.stride = block_table_stride;
+  p.width = max_blocks;
+  p.batch = batch_size;
+  p.page_size = page_size;
+  p.lens = seq_lens;
+  p.window = window_left < 0 ? -1 : window_left;
+  p.sinks = num_sink_tokens;
+  p.refs = ref_counts;
+  p.num_pages = num_pages;
+  p.counts = counts;
+  return launch_chain(release_pages_kernel, dim3(batch_size), dim3(kReleaseThreads), 0, s, p);
+}
+
+int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                      int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                      const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                      const int32_t* seq_lens, const int32_t* parents, int32_t num_sequences,
+                      int32_t page_size, int32_t* ref_counts, int32_t* out_block_tables,
+                      int64_t out_stride, int32_t* out_seq_lens, int32_t* counts,
+                      int32_t* workspace, void* stream) {
+  int st = check_pool(pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
+                      num_pages);
+  if (st != PA_OK) return st;
+  st = check_tables(block_tables, block_table_stride, max_blocks, num_sequences, page_size);
+  if (st != PA_OK) return st;
+  st = check_tables(out_block_tables, out_stride, max_blocks, num_sequences, page_size);
+  if (st != PA_OK) return st;
+  if (counts == nullptr || ref_counts == nullptr || max_blocks <= 0) return PA_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (num_sequences == 0)
+    return cudaMemsetAsync(counts, 0, 3 * sizeof(int32_t), s) == cudaSuccess ? PA_OK : PA_ERR_CUDA;
+  if (seq_lens == nullptr || parents == nullptr || out_seq_lens == nullptr ||
+      workspace == nullptr || out_block_tables == block_tables)
+    return PA_ERR_INVALID_ARGUMENT;
+  ForkSeqParams p;
+  p.tables = block_tables;
+  p.stride = block_table_stride;
+  p.width = max_blocks;
+  p.rows = num_sequences;
+  p.page_size = page_size;
+  p.lens = seq_lens;
+  p.parents = parents;
+  p.refs = ref_counts;
+  p.num_pages = num_pages;
+  p.out_tables = out_block_tables;
+  p.out_stride = out_stride;
+  p.out_lens = out_seq_lens;
+  p.counts = counts;
+  p.avail = workspace;
+  p.dst = workspace + num_sequences;
+  p.state = workspace + 2 * static_cast<int64_t>(num_sequences);
+  st = launch_chain(fork_rows_kernel, dim3(num_sequences), dim3(kForkThreads), 0, s, p);
+  if (st != PA_OK) return st;
+  st = launch_chain(fork_assign_kernel, dim3(1), dim3(kScanThreads), 0, s, p);
+  if (st != PA_OK || num_layers == 0 || page_bytes == 0) return st;
+  return launch_copy_pages(pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
+                           p.state, p.dst, counts, num_sequences, s);
+}
+
+int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                     int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                     int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                     const int32_t* seq_lens, int32_t batch_size, int32_t page_size,
+                     int32_t* ref_counts, int32_t* remap, int32_t* counts, int32_t* workspace,
+                     void* stream) {
+  int st = check_pool(pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
+                      num_pages);
+  if (st != PA_OK) return st;
+  st = check_tables(block_tables, block_table_stride, max_blocks, batch_size, page_size);
+  if (st != PA_OK) return st;
+  if (counts == nullptr || ref_counts == nullptr || remap == nullptr || workspace == nullptr ||
+      (batch_size > 0 && seq_lens == nullptr))
+    return PA_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CompactParams c;
+  c.refs = ref_counts;
+  c.num_pages = num_pages;
+  c.remap = remap;
+  c.src = workspace;
+  c.dst = workspace + num_pages / 2 + 1;
+  c.counts = counts;
+  st = launch_chain(compact_plan_kernel, dim3(1), dim3(kScanThreads), 0, s, c);
+  if (st != PA_OK) return st;
+  if (batch_size > 0) {
+    RemapParams r;
+    r.tables = block_tables;
+    r.stride = block_table_stride;
+    r.width = max_blocks;
+    r.batch = batch_size;
+    r.page_size = page_size;
+    r.lens = seq_lens;
+    r.remap = remap;
+    r.num_pages = num_pages;
+    r.counts = counts;
+    st = launch_chain(remap_tables_kernel, dim3(batch_size), dim3(kReleaseThreads), 0, s, r);
+    if (st != PA_OK) return st;
+  }
+  if (num_layers == 0 || page_bytes == 0) return PA_OK;
+  return launch_copy_pages(pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
+                           c.src, c.dst, counts + 1, num_pages / 2, s);
+}
+
+}  // extern "C"
+
+namespace {
+
+// Vectors per thread of the chunk pass: as many as leave enough CTAs.
+template <typename T>
+int beam_vectors(int64_t rows, int vocab, int sms) {
+  for (int v = 8; v > 1; v /= 2) {
+    const int ch = kBeamThreads * BeamVec<T>::N * v;
+    if (rows * ((vocab + ch - 1) / ch) >= 4 * static_cast<int64_t>(sms)) return v;
+  }
+  return 1;
+}
+
+template <typename T>
+int beam_chunk_elements(int64_t rows, int vocab, int sms) {
+  return kBeamThreads * BeamVec<T>::N * beam_vectors<T>(rows, vocab, sms);
+}
+
+int beam_chunks(int dtype, int64_t rows, int vocab, int sms) {
+  const int ch = dtype == PA_DTYPE_F32 ? beam_chunk_elements<float>(rows, vocab, sms)
+                                       : beam_chunk_elements<__half>(rows, vocab, sms);
+  return (vocab + ch - 1) / ch;
+}
+
+struct BeamWsLayout {
+  size_t sum, key, max, total;
+};
+
+BeamWsLayout beam_ws_layout(int64_t rows, int chunks, int k) {
+  BeamWsLayout L;
+  const size_t n = static_cast<size_t>(rows) * chunks;
+  L.sum = 0;
+  L.key = align256(n * sizeof(double));
+  L.max = L.key + align256(n * k * sizeof(uint64_t));
+  L.total = L.max + align256(n * sizeof(float));
+  return L;
+}
+
+template <typename T>
+int launch_beam(const BeamParams& p, int vectors, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.batch) * p.beams * p.chunks), block(kBeamThreads);
+  switch (vectors) {
+    case 8: return launch_chain(beam_chunk_kernel<T, 8>, grid, block, 0, s, p);
+    case 4: return launch_chain(beam_chunk_kernel<T, 4>, grid, block, 0, s, p);
+    case 2: return launch_chain(beam_chunk_kernel<T, 2>, grid, block, 0, s, p);
+    default: return launch_chain(beam_chunk_kernel<T, 1>, grid, block, 0, s, p);
+  }
+}
+
+int check_beam(int batch, int beams, int vocab, int k, int dtype) {
+  if (batch < 0 || beams <= 0 || vocab <= 0 || k <= 0) return PA_ERR_INVALID_ARGUMENT;
+  if (dtype != PA_DTYPE_F32 && !valid_dtype(dtype)) return PA_ERR_UNSUPPORTED;
+  const int64_t flat = static_cast<int64_t>(beams) * vocab;
+  if (k > flat) return PA_ERR_INVALID_ARGUMENT;
+  if (k > kBeamMaxK || beams > kBeamMaxBeams || vocab > kBeamMaxVocab) return PA_ERR_UNSUPPORTED;
+  return PA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pa_beam_select_workspace_bytes(int32_t batch_size, int32_t num_beams, int32_t vocab_size,
+                                      int32_t num_candidates, int32_t dtype) {
+  if (check_beam(batch_size, num_beams, vocab_size, num_candidates, dtype) != PA_OK) return 0;
+  const int dev = current_device();
+  const int sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
+  const int64_t rows = static_cast<int64_t>(batch_size) * num_beams;
+  return beam_ws_layout(rows, beam_chunks(dtype, rows, vocab_size, sms), num_candidates).total;
+}
+
+int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_stride_w,
+                   const float* scores, int64_t scores_stride_b, int32_t batch_size,
+                   int32_t num_beams, int32_t vocab_size, int32_t num_candidates, int32_t dtype,
+                   float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  const int st = check_beam(batch_size, num_beams, vocab_size, num_candidates, dtype);
+  if (st != PA_OK) return st;
+  if (batch_size == 0) return PA_OK;
+  if (logits == nullptr || scores == nullptr || out_scores == nullptr || out_parents == nullptr ||
+      out_tokens == nullptr || workspace == nullptr || !aligned16(workspace) ||
+      reinterpret_cast<uintptr_t>(logits) % (dtype == PA_DTYPE_F32 ? 4 : 2))
+    return PA_ERR_INVALID_ARGUMENT;
+  const int dev = current_device();
+  const int sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
+  const int64_t rows = static_cast<int64_t>(batch_size) * num_beams;
+  const int chunks = beam_chunks(dtype, rows, vocab_size, sms);
+  if (rows * chunks > 0x7fffffffLL) return PA_ERR_UNSUPPORTED;
+  const BeamWsLayout L = beam_ws_layout(rows, chunks, num_candidates);
+  if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  BeamParams p;
+  p.logits = logits;
+  p.stride_b = logits_stride_b;
+  p.stride_w = logits_stride_w;
+  p.scores = scores;
+  p.score_stride = scores_stride_b;
+  p.batch = batch_size;
+  p.beams = num_beams;
+  p.vocab = vocab_size;
+  p.k = num_candidates;
+  p.chunks = chunks;
+  p.part_max = reinterpret_cast<float*>(ws + L.max);
+  p.part_sum = reinterpret_cast<double*>(ws + L.sum);
+  p.part_key = reinterpret_cast<uint64_t*>(ws + L.key);
+  p.out_scores = out_scores;
+  p.out_parents = out_parents;
+  p.out_tokens = out_tokens;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int rc;
+  if (dtype == PA_DTYPE_F32)
+    rc = launch_beam<float>(p, beam_vectors<float>(rows, vocab_size, sms), s);
+  else if (dtype == PA_DTYPE_BF16)
+    rc = launch_beam<__nv_bfloat16>(p, beam_vectors<__nv_bfloat16>(rows, vocab_size, sms), s);
+  else
+    rc = launch_beam<__half>(p, beam_vectors<__half>(rows, vocab_size, sms), s);
+  if (rc != PA_OK) return rc;
+  const size_t smem = static_cast<size_t>(num_beams) * 12 + 8;
+  return launch_chain(beam_join_kernel, dim3(batch_size), dim3(kBeamThreads), smem, s, p);
 }
 
 int pa_qkv_rope_append(const void* x, int64_t x_stride, const void* weight, int64_t w_stride,
