@@ -264,7 +264,7 @@ int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
  * larger logit, then the lowest token: out_scores (fp32), out_parents
  * (b * num_beams + w, a row of pa_fork_sequences), out_tokens, each
  * [batch, num_candidates].
- * A NaN logit counts as -inf, +inf as the largest finite value; beams whose
+ * A NaN logit counts as -inf, +inf as its type's largest value; beams whose
  * score is -inf or NaN and rows without a finite logit score -inf. */
 size_t pa_beam_select_workspace_bytes(int32_t batch_size, int32_t num_beams, int32_t vocab_size,
                                       int32_t num_candidates, int32_t dtype);

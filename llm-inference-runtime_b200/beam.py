@@ -9,18 +9,25 @@ continuations of each request's beams, and the cache following them
 
 from __future__ import annotations
 
+import functools
 from typing import Dict, Tuple
 
 import torch
 
 from . import _lib, pages
-from .flashinfer_api import _after
+from .flashinfer_api import _after, _device_guard, _stream
 
 _DTYPES = {torch.float16: _lib.PA_DTYPE_F16, torch.bfloat16: _lib.PA_DTYPE_BF16,
            torch.float32: _lib.PA_DTYPE_F32}
 MAX_CANDIDATES = 32
 MAX_BEAMS = 256
 MAX_VOCAB = 2 ** 24
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device_index: int, *sizes: int) -> int:
+    """A function of the sizes and the device's SM count alone."""
+    return _lib.load().pa_beam_select_workspace_bytes(*sizes)
 
 
 def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int
@@ -57,19 +64,18 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
         scores = scores.contiguous()
     device = logits.device
     dtype = _DTYPES[logits.dtype]
-    out = torch.empty((3, batch, n), dtype=torch.int32, device=device)
-    best, parents, tokens = out[0].view(torch.float32), out[1], out[2]
+    best = torch.empty((batch, n), dtype=torch.float32, device=device)
+    parents = torch.empty((batch, n), dtype=torch.int32, device=device)
+    tokens = torch.empty_like(parents)
     if batch == 0:
         return best, parents, tokens
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        size = lib.pa_beam_select_workspace_bytes(batch, beams, vocab, n, dtype)
+    with _device_guard(device):
+        size = _workspace_bytes(device.index, batch, beams, vocab, n, dtype)
         ws = torch.empty(size, dtype=torch.uint8, device=device)
-        _lib.check(lib.pa_beam_select(
+        _lib.check(_lib.load().pa_beam_select(
             logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(),
             scores.stride(0), batch, beams, vocab, n, dtype, best.data_ptr(), parents.data_ptr(),
-            tokens.data_ptr(), ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream),
-            "beam_search_select")
+            tokens.data_ptr(), ws.data_ptr(), size, _stream()), "beam_search_select")
         _after("beam_search_select")
     return best, parents, tokens
 

@@ -13,12 +13,14 @@
 // request.
 //
 // Chunk pass: a CTA holds a chunk in registers (all its loads in flight at
-// once), takes the chunk's maximum and sum from them, and finds a threshold
-// that K of its elements reach: in each warp the K-th largest of the threads'
-// maxima, the largest of those over the warps. Few elements pass it; they are
-// ranked by counting. Keys are (value, lowest index first) in 64 bits, unique,
-// so equal logits cost nothing extra; more than kBeamCap elements pass only
-// for inputs laid out against the threads' order, and then K rounds of a
+// once) and takes the chunk's maximum and sum from them. Of its 256 threads'
+// maxima each warp's four best are looked at; the K-th of those 32 is a
+// threshold that at least K logits reach and few others do. The threads whose
+// maximum reaches it (about K of 256) have their logits read again, a word per
+// lane, and what passes is ranked by counting. Many more reach it only when
+// many are equal to it (masked or constant rows): then the ones above it and,
+// in index order, as many equal ones as are missing are taken. If more than
+// kBeamCap lie above it (a layout against the threads' order), K rounds of a
 // block-wide maximum give the same result.
 #pragma once
 
@@ -28,9 +30,10 @@ namespace pa {
 
 constexpr int kBeamThreads = 256;
 constexpr int kBeamWarps = kBeamThreads / 32;
-constexpr int kBeamMaxK = 32;   // the K-th of a warp's 32 maxima
+constexpr int kBeamMaxK = 32;   // the threshold looks at 32 maxima
 constexpr int kBeamMaxBeams = 256;      // JoinKey's 8 bits
 constexpr int kBeamMaxVocab = 1 << 24;  // and 24
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kBeamCap = 1024;  // elements ranked by counting
 
 struct BeamParams {
@@ -39,8 +42,8 @@ struct BeamParams {
   const float* scores;         // [batch, beams]
   int64_t score_stride;
   int32_t batch, beams, vocab, k, chunks;
-  float* part_max;    // [rows, chunks]
-  double* part_sum;   // [rows, chunks]: sum of exp(x - part_max)
+  double* part_off;   // [rows, chunks]: off, about max * log2(e); -inf: nothing finite
+  double* part_sum;   // [rows, chunks]: sum of 2^(x log2(e) - off)
   uint64_t* part_key;  // [rows, chunks, k]: best first, 0: none
   float* out_scores;  // [batch, k]
   int32_t* out_parents;
@@ -64,12 +67,6 @@ __device__ __forceinline__ double order_value64(uint64_t k) {
       static_cast<long long>(k ^ ((k >> 63) ? 0x8000000000000000ULL : 0xffffffffffffffffULL)));
 }
 
-// NaN counts as -inf, +inf as the largest finite value; -0 becomes +0.
-__device__ __forceinline__ float clean(float x) {
-  x = x != x ? -INFINITY : x;
-  return fminf(x, 3.402823466e38f) + 0.f;
-}
-
 // (value, index) as one key: larger value first, then the lower index.
 __device__ __forceinline__ uint64_t beam_key(float x, int idx) {
   return (static_cast<uint64_t>(order_bits(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(idx));
@@ -91,42 +88,29 @@ __device__ __forceinline__ JoinKey shfl_xor_key(const JoinKey& k, int m) {
   return JoinKey{__shfl_xor_sync(0xffffffffu, k.score, m),
                  __shfl_xor_sync(0xffffffffu, k.rest, m)};
 }
-__device__ __forceinline__ uint64_t shfl_key(uint64_t k, int l) {
-  return __shfl_sync(0xffffffffu, k, l);
-}
-__device__ __forceinline__ JoinKey shfl_key(const JoinKey& k, int l) {
-  return JoinKey{__shfl_sync(0xffffffffu, k.score, l), __shfl_sync(0xffffffffu, k.rest, l)};
-}
-
-// The warp's 32 keys in descending order over the lanes (bitonic network).
-template <typename K>
-__device__ __forceinline__ K warp_sort_desc(K key, int lane) {
+// Threshold that at least k <= 32 of the threads' keys reach, or 0 if fewer
+// than k threads have one (0: none); *top receives the largest key. One
+// barrier. s_four: four keys per warp.
+__device__ __forceinline__ uint32_t block_threshold(uint32_t key, int k, uint32_t* s_four, int lane,
+                                                    int wid, uint32_t* top) {
+  uint32_t left = key;
 #pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      const K other = shfl_xor_key(key, step);
-      const bool desc = (lane & size) == 0;  // size 32: all descending
-      const bool low = (lane & step) == 0;
-      const bool take_max = low == desc;
-      if (take_max ? other > key : key > other) key = other;
-    }
-  return key;
-}
-
-// Threshold that at least k of the block's elements reach, from each thread's
-// best key (zero: none): see the header. s_key: one key per warp.
-template <typename K>
-__device__ __forceinline__ K block_threshold(K best, int k, K* s_key, int lane, int wid) {
-  const K sorted = warp_sort_desc(best, lane);
-  const K kth = shfl_key(sorted, k - 1);
-  if (lane == 0) s_key[wid] = kth;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = __reduce_max_sync(0xffffffffu, left);
+    if (lane == 0) s_four[wid * 4 + i] = m;
+    const uint32_t who = __ballot_sync(0xffffffffu, left == m);
+    if (lane == __ffs(who) - 1) left = 0;
+  }
   __syncthreads();
-  K t = s_key[0];
+  const uint32_t mine = s_four[lane];
+  int reach = 0;  // how many of the 32 are at least mine
 #pragma unroll
-  for (int w = 1; w < kBeamWarps; ++w)
-    if (s_key[w] > t) t = s_key[w];
-  return t;
+  for (int i = 0; i < 8; ++i) {
+    const uint4 o = reinterpret_cast<const uint4*>(s_four)[i];
+    reach += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
+  }
+  *top = __reduce_max_sync(0xffffffffu, mine);
+  return __reduce_max_sync(0xffffffffu, reach >= k ? mine : 0u);
 }
 
 template <typename K>
@@ -146,27 +130,67 @@ __device__ __forceinline__ K block_max(K best, K* s_key, int lane, int wid) {
   return t;
 }
 
-// Eight 16-bit or four 32-bit logits of a thread, as they lie in memory.
+// Logits as they lie in memory, one 32-bit word at a time: one fp32 or two
+// 16-bit values, whose maxima and comparisons work on both at once.
 template <typename T>
-struct BeamVec {
-  static constexpr int N = 16 / sizeof(T);
-  uint4 raw;
-  __device__ __forceinline__ float at(int i) const;
+struct BeamWord;
+
+template <>
+struct BeamWord<float> {
+  static constexpr int N = 1;
+  static constexpr uint32_t kNone = 0xff800000u;  // -inf
+  static constexpr float kMost = 3.402823466e38f;
+  // NaN becomes -inf, +inf the largest finite value
+  static __device__ __forceinline__ uint32_t clean(uint32_t w) {
+    return __float_as_uint(fminf(fmaxf(__uint_as_float(w), -INFINITY), 3.402823466e38f));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float at(uint32_t w, int) { return __uint_as_float(w); }
+  // the word's first n values, -inf for the others
+  static __device__ __forceinline__ uint32_t first(uint32_t w, int n) { return n > 0 ? w : kNone; }
+};
+
+template <typename T, typename T2>
+struct BeamWord16 {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ T2 val(uint32_t w) { return *reinterpret_cast<const T2*>(&w); }
+  static __device__ __forceinline__ uint32_t raw(T2 v) {
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    return raw(__hmax2(val(a), val(b)));
+  }
 };
 template <>
-__device__ __forceinline__ float BeamVec<float>::at(int i) const {
-  return __uint_as_float(reinterpret_cast<const uint32_t*>(&raw)[i]);
-}
+struct BeamWord<__nv_bfloat16> : BeamWord16<__nv_bfloat16, __nv_bfloat162> {
+  static constexpr uint32_t kNone = 0xff80ff80u;
+  static constexpr float kMost = 3.3895313892515355e38f;
+  static __device__ __forceinline__ uint32_t first(uint32_t w, int n) {
+    return n >= 2 ? w : n == 1 ? (w & 0xffffu) | (kNone << 16) : kNone;
+  }
+  static __device__ __forceinline__ uint32_t clean(uint32_t w) {
+    return raw(__hmin2(__hmax2(val(w), val(kNone)), val(0x7f7f7f7fu)));
+  }
+  static __device__ __forceinline__ float at(uint32_t w, int i) {
+    return __uint_as_float(i ? w & 0xffff0000u : w << 16);
+  }
+};
 template <>
-__device__ __forceinline__ float BeamVec<__nv_bfloat16>::at(int i) const {
-  const uint32_t w = reinterpret_cast<const uint32_t*>(&raw)[i >> 1];
-  return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-}
-template <>
-__device__ __forceinline__ float BeamVec<__half>::at(int i) const {
-  const uint32_t w = reinterpret_cast<const uint32_t*>(&raw)[i >> 1];
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w >> 16 : w)));
-}
+struct BeamWord<__half> : BeamWord16<__half, __half2> {
+  static constexpr uint32_t kNone = 0xfc00fc00u;
+  static constexpr float kMost = 65504.f;
+  static __device__ __forceinline__ uint32_t first(uint32_t w, int n) {
+    return n >= 2 ? w : n == 1 ? (w & 0xffffu) | (kNone << 16) : kNone;
+  }
+  static __device__ __forceinline__ uint32_t clean(uint32_t w) {
+    return raw(__hmin2(__hmax2(val(w), val(kNone)), val(0x7bff7bffu)));
+  }
+  static __device__ __forceinline__ float at(uint32_t w, int i) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(i ? w >> 16 : w)));
+  }
+};
 
 // 16 bytes at `p` (any alignment that is a multiple of the element's), of
 // which the first `bytes` > 0 exist: the aligned 16-byte blocks that hold at
@@ -187,18 +211,26 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p, int bytes) {
   return v;
 }
 
-// One chunk of one row. Element e of vector i of thread t is logit
-// chunk * CH + (i * 256 + t) * N + e whatever the row's alignment, so equal
-// rows give equal sums.
+// One chunk of one row. Vector i of thread t holds logits chunk * CH +
+// (i * 256 + t) * N and the N - 1 after it whatever the row's alignment, so
+// equal rows give equal sums; places past the row hold -inf.
+//
+// Per logit: half an instruction of packed maxima and four for the sum (unpack,
+// fma, ex2, add). ex2 is the narrowest pipe (16 per SM and cycle). NaN needs no instruction of its
+// own: maxima and comparisons pass over it, and a thread whose sum comes out
+// NaN cleans its logits and adds them up again.
 template <typename T, int VPT>
-__global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const BeamParams p) {
-  using V = BeamVec<T>;
-  constexpr int N = V::N;
+__global__ void __launch_bounds__(kBeamThreads, 3) beam_chunk_kernel(const BeamParams p) {
+  using W = BeamWord<T>;
+  constexpr int N = 16 / sizeof(T);
   constexpr int CH = kBeamThreads * N * VPT;
+  __shared__ alignas(16) uint32_t s_four[32];
   __shared__ uint64_t s_key[kBeamWarps];
-  __shared__ double s_sum[kBeamWarps];
+  __shared__ float s_sum[kBeamWarps];
+  __shared__ int s_warp[kBeamWarps];
   __shared__ uint64_t s_cand[kBeamCap];
-  __shared__ int s_n;
+  __shared__ uint8_t s_who[kBeamThreads];
+  __shared__ int s_n, s_nwho;
   griddep_wait();
   griddep_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -206,79 +238,120 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const BeamPara
   const int b = row / p.beams, w = row - b * p.beams;
   const T* x = static_cast<const T*>(p.logits) + b * p.stride_b + w * p.stride_w;
   const int base = chunk * CH, K = p.k;
-  if (tid == 0) s_n = 0;
+  if (tid == 0) s_n = s_nwho = 0;
   // a beam without a score continues nothing: all its logits count as -inf
   const float c0 = __ldg(p.scores + b * p.score_stride + w);
   const bool dead = !(c0 > -INFINITY);
 
-  V v[VPT];
+  // vector i of this thread, whatever its alignment; places past the row: -inf
+  auto load = [&](int i) {
+    uint4 r = make_uint4(W::kNone, W::kNone, W::kNone, W::kNone);
+    const int at = base + (i * kBeamThreads + tid) * N;
+    const int left = dead ? 0 : p.vocab - at;
+    if (left <= 0) return r;
+    r = load16_any(reinterpret_cast<const uint8_t*>(x + at),
+                   min(left, N) * static_cast<int>(sizeof(T)));
+    if (left < N) {
+      r.x = W::first(r.x, left);
+      r.y = W::first(r.y, left - W::N);
+      r.z = W::first(r.z, left - 2 * W::N);
+      r.w = W::first(r.w, left - 3 * W::N);
+    }
+    return r;
+  };
+  uint32_t v[VPT][4];
+  const bool whole = !dead && base + CH <= p.vocab &&
+                     (reinterpret_cast<uintptr_t>(x + base) & 15) == 0;
+  const uint4* src = reinterpret_cast<const uint4*>(x + base) + tid;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int at = base + (i * kBeamThreads + tid) * N;
-    const int left = p.vocab - at;
-    v[i].raw = make_uint4(0, 0, 0, 0);
-    if (left > 0)
-      v[i].raw = load16_any(reinterpret_cast<const uint8_t*>(x + at),
-                            min(left, N) * static_cast<int>(sizeof(T)));
+    const uint4 r = whole ? __ldcs(src + i * kBeamThreads) : load(i);
+    v[i][0] = r.x;
+    v[i][1] = r.y;
+    v[i][2] = r.z;
+    v[i][3] = r.w;
   }
-  auto value = [&](int i, int e) { return dead ? -INFINITY : clean(v[i].at(e)); };
-  // elements of vector i inside the row, and their place in it
-  auto count = [&](int i) { return p.vocab - base - (i * kBeamThreads + tid) * N; };
-  auto index = [&](int i, int e) { return base + (i * kBeamThreads + tid) * N + e; };
-
-  // the thread's best element, the lowest index among equal ones
-  float best = -INFINITY;
-  int best_at = -1;
+  auto clean_all = [&]() {
 #pragma unroll
-  for (int i = VPT - 1; i >= 0; --i) {
-    const int n = count(i);
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-    for (int e = N - 1; e >= 0; --e) {
-      const float f = value(i, e);
-      if (e < n && f >= best) {
-        best = f;
-        best_at = index(i, e);
-      }
-    }
+      for (int q = 0; q < 4; ++q) v[i][q] = W::clean(v[i][q]);
+  };
+  auto thread_max = [&]() {
+    uint32_t m = W::kNone;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m = W::max2(m, v[i][q]);
+    return W::N == 2 ? fmaxf(W::at(m, 0), W::at(m, 1)) : W::at(m, 0);
+  };
+  float best = thread_max();
+  if (best == INFINITY) {
+    clean_all();
+    best = thread_max();
   }
-  const uint64_t mine = best_at >= 0 ? beam_key(best, best_at) : 0;
-  const uint64_t least = block_threshold<uint64_t>(mine, K, s_key, lane, wid);
-  const uint64_t top = block_max<uint64_t>(mine, s_key, lane, wid);
-  const float m = order_value(static_cast<uint32_t>(top >> 32));  // the chunk is not empty
+  // 0: no logit here. (+ 0.f: -0 and +0 are one value)
+  const uint32_t mine = base + tid * N < p.vocab ? order_bits(best + 0.f) : 0u;
+  uint32_t top;
+  const uint32_t least = block_threshold(mine, K, s_four, lane, wid, &top);
+  const float m = order_value(top);  // the chunk is not empty
+  // (s_nwho was set before the barrier above)
+  if (mine >= least && mine != 0) s_who[atomicAdd(&s_nwho, 1)] = static_cast<uint8_t>(tid);
 
-  // this chunk's sum of exp(x - m)
-  double sum = 0.0;
-  {
+  // this chunk's sum of 2^(x log2(e) - off), off = m log2(e) rounded: the join
+  // takes the same off, so its rounding cancels
+  const float off = m * kLog2e;
+  const bool huge = fabsf(m) > 1e30f;  // the product may overflow; x - m does as well there
+  float sum = 0.f;
+  if (m != -INFINITY && !huge) {
     float part[4] = {0.f, 0.f, 0.f, 0.f};
-    if (m != -INFINITY) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int n = count(i);
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          // x - m first: exact near the maximum, where the sum's weight is
-          const float t = ex2((value(i, e) - m) * 1.4426950408889634f);
-          part[e & 3] += e < n ? t : 0.f;
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < W::N; ++e)
+          part[(q * W::N + e) & 3] += ex2(fmaf(W::at(v[i][q], e), kLog2e, -off));
+    sum = (part[0] + part[1]) + (part[2] + part[3]);
+  }
+  if (m != -INFINITY && (huge || sum != sum)) {
+    // rare: from memory again, with NaN as -inf
+    sum = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < VPT; ++i) {
+      const uint4 r = load(i);
+      const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < W::N; ++e) {
+          const float f = W::at(word[q], e);
+          sum += ex2(huge ? (f - m) * kLog2e : fmaf(f, kLog2e, -off));
         }
-      }
     }
-    sum = (static_cast<double>(part[0]) + part[1]) + (static_cast<double>(part[2]) + part[3]);
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[wid] = sum;
+  __syncthreads();
 
-  // the elements that reach the threshold
-  if (mine >= least && mine != 0) {
+  // the logits that reach the threshold, in any order: lane l reads word l of
+  // a thread's VPT * 4
+  auto index = [&](int i, int q, int e) {
+    return base + (i * kBeamThreads + tid) * N + q * W::N + e;
+  };
+  const int nwho = s_nwho;
+  if (!dead && lane < VPT * 4) {
+    for (int k = wid; k < nwho; k += kBeamWarps) {
+      const int at = base + ((lane >> 2) * kBeamThreads + s_who[k]) * N + (lane & 3) * W::N;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int n = count(i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint64_t key = beam_key(value(i, e), index(i, e));
-        if (e < n && key >= least) {
-          const int at = atomicAdd(&s_n, 1);
-          if (at < kBeamCap) s_cand[at] = key;
+      for (int e = 0; e < W::N; ++e) {
+        if (at + e >= p.vocab) continue;
+        const float raw = static_cast<float>(__ldg(x + at + e));
+        const float f = fminf(raw, W::kMost) + 0.f;
+        if (raw == raw && order_bits(f) >= least) {
+          const int n = atomicAdd(&s_n, 1);
+          if (n < kBeamCap) s_cand[n] = beam_key(f, at + e);
         }
       }
     }
@@ -288,11 +361,68 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const BeamPara
     double total = 0.0;
 #pragma unroll
     for (int k = 0; k < kBeamWarps; ++k) total += s_sum[k];
-    p.part_max[blockIdx.x] = m;
+    p.part_off[blockIdx.x] = huge ? m * 1.4426950408889634 : off;
     p.part_sum[blockIdx.x] = total;
   }
   uint64_t* out = p.part_key + static_cast<int64_t>(blockIdx.x) * K;
-  const int n = s_n;
+  int n = s_n;
+  if (n > kBeamCap || least <= order_bits(-INFINITY)) {
+    // many equal the threshold (or NaN counts as -inf, which nothing above
+    // has seen): from memory again, first those above it
+    __syncthreads();
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    const uint32_t equal = max(least, order_bits(-INFINITY));
+#pragma unroll 1
+    for (int i = 0; i < VPT; ++i) {
+      const uint4 r = load(i);
+      const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < W::N; ++e) {
+          const float f = W::at(word[q], e) + 0.f;
+          if (order_bits(f) > equal && index(i, q, e) < p.vocab) {
+            const int at = atomicAdd(&s_n, 1);
+            if (at < kBeamCap) s_cand[at] = beam_key(f, index(i, q, e));
+          }
+        }
+    }
+    __syncthreads();
+    n = s_n;
+    // then the first equal ones: vector i of all threads comes before i + 1
+#pragma unroll 1
+    for (int i = 0; i < VPT && n < K; ++i) {  // n: the same for every thread
+      const uint4 r = load(i);
+      const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
+      uint32_t mask = 0;  // which of the vector's logits are equal
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < W::N; ++e)
+          if (order_bits(W::at(word[q], e) + 0.f) == equal && index(i, q, e) < p.vocab)
+            mask |= 1u << (q * W::N + e);
+      int incl = __popc(mask);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      if (lane == 31) s_warp[wid] = incl;
+      __syncthreads();
+      int at = n + incl - __popc(mask), total = 0;
+#pragma unroll
+      for (int k = 0; k < kBeamWarps; ++k) {
+        at += k < wid ? s_warp[k] : 0;
+        total += s_warp[k];
+      }
+      const uint64_t value = static_cast<uint64_t>(equal) << 32;
+      for (; mask != 0 && at < K; mask &= mask - 1, ++at)
+        s_cand[at] = value | (0xffffffffu - static_cast<uint32_t>(index(i, 0, __ffs(mask) - 1)));
+      n = min(n + total, K);
+      __syncthreads();  // s_warp may be written again; s_cand is complete
+    }
+  }
   if (n <= kBeamCap) {
     for (int i = tid; i < n; i += kBeamThreads) {
       const uint64_t key = s_cand[i];
@@ -300,20 +430,24 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const BeamPara
       for (int j = 0; j < n; ++j) rank += s_cand[j] > key;
       if (rank < K) out[rank] = key;
     }
-    for (int i = n + tid; i < K; i += kBeamThreads) out[i] = 0;  // fewer elements than K
+    for (int i = n + tid; i < K; i += kBeamThreads) out[i] = 0;  // fewer logits than K
     return;
   }
   uint64_t last = ~0ULL;
+#pragma unroll 1
   for (int k = 0; k < K; ++k) {
     uint64_t next = 0;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < VPT; ++i) {
-      const int left = count(i);
+      const uint4 r = load(i);
+      const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint64_t key = beam_key(value(i, e), index(i, e));
-        if (e < left && key < last && key > next) next = key;
-      }
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < W::N; ++e) {
+          const uint64_t key = beam_key(W::at(word[q], e) + 0.f, index(i, q, e));
+          if (index(i, q, e) < p.vocab && key < last && key > next) next = key;
+        }
     }
     last = block_max<uint64_t>(next, s_key, lane, wid);
     if (tid == 0) out[k] = last;
@@ -325,6 +459,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const BeamParam
   extern __shared__ uint8_t beam_smem[];
   float* s_lse = reinterpret_cast<float*>(beam_smem);  // [beams]
   double* s_base = reinterpret_cast<double*>(beam_smem + ((p.beams * 4 + 7) & ~7));  // [beams]
+  __shared__ alignas(16) uint32_t s_four[32];
   __shared__ JoinKey s_key[kBeamWarps];
   __shared__ JoinKey s_cand[kBeamCap];
   __shared__ int s_n;
@@ -335,22 +470,21 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const BeamParam
   if (tid == 0) s_n = 0;
   for (int w = wid; w < p.beams; w += kBeamWarps) {
     const int64_t at = (static_cast<int64_t>(b) * p.beams + w) * C;
-    float m = -INFINITY;
-    for (int c = lane; c < C; c += 32) m = fmaxf(m, __ldcg(p.part_max + at + c));
+    double m = -INFINITY;
+    for (int c = lane; c < C; c += 32) m = fmax(m, __ldcg(p.part_off + at + c));
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    for (int off = 16; off > 0; off >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, off));
     double sum = 0.0;
     for (int c = lane; c < C; c += 32) {
-      const float mc = __ldcg(p.part_max + at + c);
-      if (mc != -INFINITY)
-        sum += exp(static_cast<double>(mc) - m) * __ldcg(p.part_sum + at + c);
+      const double mc = __ldcg(p.part_off + at + c);
+      if (mc != -INFINITY) sum += exp2(mc - m) * __ldcg(p.part_sum + at + c);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (lane == 0) {
       const float c = p.scores[b * p.score_stride + w];
       const bool dead = m == -INFINITY || !(c > -INFINITY);  // continues nothing
-      s_lse[w] = dead ? 0.f : static_cast<float>(m + log(sum));
+      s_lse[w] = dead ? 0.f : static_cast<float>((m + log2(sum)) * 0.6931471805599453);
       s_base[w] = dead ? -INFINITY : static_cast<double>(fminf(c, 3.402823466e38f));
     }
   }
@@ -371,16 +505,16 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const BeamParam
     return JoinKey{order_bits64(s), (static_cast<uint64_t>(255 - w) << 56) |
                                         ((key >> 32) << 24) | (0xffffffu - token)};
   };
-  JoinKey best{0, 0};
-  for (int i = tid; i < total; i += kBeamThreads) {
-    const JoinKey c = candidate(i);
-    if (c > best) best = c;
-  }
-  const JoinKey least = block_threshold<JoinKey>(best, K, s_key, lane, wid);
-  if (!(least > best) && best.score != 0) {
+  uint64_t best = 0;
+  for (int i = tid; i < total; i += kBeamThreads) best = max(best, candidate(i).score);
+  // (the upper half of the score's bits is threshold enough)
+  uint32_t top;
+  const uint32_t least = block_threshold(static_cast<uint32_t>(best >> 32), K, s_four, lane, wid,
+                                         &top);
+  if (best != 0 && best >> 32 >= least) {
     for (int i = tid; i < total; i += kBeamThreads) {
       const JoinKey c = candidate(i);
-      if (c.score != 0 && !(least > c)) {
+      if (c.score != 0 && c.score >> 32 >= least) {
         const int at = atomicAdd(&s_n, 1);
         if (at < kBeamCap) s_cand[at] = c;
       }

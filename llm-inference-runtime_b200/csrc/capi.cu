@@ -776,7 +776,7 @@ namespace {
 template <typename T>
 int beam_vectors(int64_t rows, int vocab, int sms) {
   for (int v = 8; v > 1; v /= 2) {
-    const int ch = kBeamThreads * BeamVec<T>::N * v;
+    const int ch = kBeamThreads * static_cast<int>(16 / sizeof(T)) * v;
     if (rows * ((vocab + ch - 1) / ch) >= 4 * static_cast<int64_t>(sms)) return v;
   }
   return 1;
@@ -784,7 +784,7 @@ int beam_vectors(int64_t rows, int vocab, int sms) {
 
 template <typename T>
 int beam_chunk_elements(int64_t rows, int vocab, int sms) {
-  return kBeamThreads * BeamVec<T>::N * beam_vectors<T>(rows, vocab, sms);
+  return kBeamThreads * static_cast<int>(16 / sizeof(T)) * beam_vectors<T>(rows, vocab, sms);
 }
 
 int beam_chunks(int dtype, int64_t rows, int vocab, int sms) {
@@ -794,16 +794,16 @@ int beam_chunks(int dtype, int64_t rows, int vocab, int sms) {
 }
 
 struct BeamWsLayout {
-  size_t sum, key, max, total;
+  size_t sum, off, key, total;
 };
 
 BeamWsLayout beam_ws_layout(int64_t rows, int chunks, int k) {
   BeamWsLayout L;
   const size_t n = static_cast<size_t>(rows) * chunks;
   L.sum = 0;
-  L.key = align256(n * sizeof(double));
-  L.max = L.key + align256(n * k * sizeof(uint64_t));
-  L.total = L.max + align256(n * sizeof(float));
+  L.off = align256(n * sizeof(double));
+  L.key = 2 * L.off;
+  L.total = L.key + align256(n * k * sizeof(uint64_t));
   return L;
 }
 
@@ -871,7 +871,7 @@ int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_s
   p.vocab = vocab_size;
   p.k = num_candidates;
   p.chunks = chunks;
-  p.part_max = reinterpret_cast<float*>(ws + L.max);
+  p.part_off = reinterpret_cast<double*>(ws + L.off);
   p.part_sum = reinterpret_cast<double*>(ws + L.sum);
   p.part_key = reinterpret_cast<uint64_t*>(ws + L.key);
   p.out_scores = out_scores;

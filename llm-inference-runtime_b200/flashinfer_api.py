@@ -27,6 +27,7 @@ each call synchronise and raise on device-side validation errors.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -54,12 +55,26 @@ def _as_dtype(dt) -> Optional[torch.dtype]:
     return _STR_DTYPES[str(dt).replace("torch.", "")]
 
 
+# The stream handle and the current device's number without the objects that
+# torch.cuda.current_stream() builds (3 us of a 10 us call).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_SAME_DEVICE = contextlib.nullcontext()
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_current_device())
+
+
+def _device_guard(device: torch.device):
+    """Makes `device` current for the launches of a call, where it is not."""
+    if device.index == _current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
 
 
 def _p(t: Optional[torch.Tensor]):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _i32_on(t: torch.Tensor, device: torch.device, name: str) -> torch.Tensor:
@@ -87,42 +102,38 @@ def kv_cache_desc(paged_kv_cache, kv_layout: str = "NHD") -> _lib.PagedKVCache:
     if isinstance(paged_kv_cache, torch.Tensor):
         if paged_kv_cache.dim() != 5 or paged_kv_cache.size(1) != 2:
             raise ValueError("paged_kv_cache tensor must be 5-D [num_pages, 2, ...]")
-        k = paged_kv_cache.select(1, 0)
-        v = paged_kv_cache.select(1, 1)
+        shape, stride = paged_kv_cache.shape, paged_kv_cache.stride()
+        shape, stride = shape[:1] + shape[2:], stride[:1] + stride[2:]
+        dtype = paged_kv_cache.dtype
+        k_ptr = paged_kv_cache.data_ptr()
+        v_ptr = k_ptr + paged_kv_cache.stride(1) * paged_kv_cache.element_size()
     else:
         k, v = paged_kv_cache
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError("k_cache / v_cache must be 4-D tensors of equal shape")
         if k.stride() != v.stride():
             raise ValueError("k_cache and v_cache must have the same strides")
-    if k.stride(-1) != 1:
+        shape, stride, dtype = k.shape, k.stride(), k.dtype
+        k_ptr, v_ptr = k.data_ptr(), v.data_ptr()
+    if stride[3] != 1:
         raise ValueError("the head_dim dimension of the KV cache must be contiguous")
     if kv_layout == "HND":
-        n, h, p, d = k.shape
-        head_stride, token_stride = k.stride(1), k.stride(2)
+        n, h, p, d = shape
+        head_stride, token_stride = stride[1], stride[2]
     else:
-        n, p, h, d = k.shape
-        token_stride, head_stride = k.stride(1), k.stride(2)
-    desc = _lib.PagedKVCache()
-    desc.k_base = k.data_ptr()
-    desc.v_base = v.data_ptr()
-    desc.page_stride = k.stride(0)
-    desc.head_stride = head_stride
-    desc.token_stride = token_stride
-    desc.num_pages = n
-    desc.num_kv_heads = h
-    desc.page_size = p
-    desc.head_dim = d
-    desc.dtype = _dtype_code(k.dtype)
-    return desc
+        n, p, h, d = shape
+        token_stride, head_stride = stride[1], stride[2]
+    return _lib.PagedKVCache(k_ptr, v_ptr, stride[0], head_stride, token_stride, n, h, p, d,
+                             _dtype_code(dtype))
 
 
 def _row_strides(x: torch.Tensor, name: str) -> Tuple[int, int]:
     if x.dim() != 3:
         raise ValueError(f"{name} must be 3-D [tokens, heads, head_dim]")
-    if x.stride(-1) != 1:
+    n, h, d = x.stride()
+    if d != 1:
         raise ValueError(f"{name}: head_dim must be contiguous")
-    return x.stride(0), x.stride(1)
+    return n, h
 
 
 # ----------------------------------------------------------------- indexing

@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .flashinfer_api import _after
+from .flashinfer_api import _after, _device_guard, _stream
 
 
 def _on_gpu_i32(t: torch.Tensor, name: str, dim: int) -> torch.Tensor:
@@ -66,32 +66,28 @@ def _pool(kv_pool: torch.Tensor, ref_counts: torch.Tensor):
         raise ValueError("kv_pool and ref_counts must be on one GPU")
     if pool.size(1) != ref_counts.numel():
         raise ValueError("ref_counts must hold one count per page of kv_pool")
-    page = pool.size(2) * pool.size(3) * pool.size(4) * pool.size(5)
-    at = 1
-    for i in (5, 4, 3, 2):  # a page of a layer is one contiguous block
-        if pool.size(i) > 1 and pool.stride(i) != at:
-            raise ValueError("each page of a layer must be one contiguous block")
-        at *= pool.size(i)
-    if (pool.size(1) > 1 and pool.stride(1) < page) or (
-            pool.size(0) > 1 and pool.stride(0) < page):
-        raise ValueError("the pages of kv_pool must not overlap")
-    es = pool.element_size()
-    return (pool.data_ptr(), pool.stride(0) * es, pool.size(0), max(pool.stride(1), page) * es,
-            page * es, pool.size(1))
-
-
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    size, stride, es = pool.shape, pool.stride(), pool.element_size()
+    page = size[2] * size[3] * size[4] * size[5]
+    if not pool.is_contiguous():
+        at = 1
+        for i in (5, 4, 3, 2):  # a page of a layer is one contiguous block
+            if size[i] > 1 and stride[i] != at:
+                raise ValueError("each page of a layer must be one contiguous block")
+            at *= size[i]
+        if (size[1] > 1 and stride[1] < page) or (size[0] > 1 and stride[0] < page):
+            raise ValueError("the pages of kv_pool must not overlap")
+    return (pool.data_ptr(), stride[0] * es, size[0], max(stride[1], page) * es, page * es,
+            size[1])
 
 
 def _release(what, block_tables, seq_lens, ref_counts, page_size, window_left, sinks):
     device = _state(block_tables, seq_lens, ref_counts)
     counts = torch.empty(3, dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
+    with _device_guard(device):
         _lib.check(_lib.load().pa_release_pages(
             block_tables.data_ptr(), _row_stride(block_tables), block_tables.size(1),
             seq_lens.data_ptr(), seq_lens.numel(), int(page_size), window_left, sinks,
-            ref_counts.data_ptr(), ref_counts.numel(), counts.data_ptr(), _stream(device)), what)
+            ref_counts.data_ptr(), ref_counts.numel(), counts.data_ptr(), _stream()), what)
         _after(what)
     return counts
 
@@ -156,12 +152,12 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
     # lengths and counts that go back, then the kernels' scratch
     ints = torch.empty(4 * rows + 3, dtype=torch.int32, device=device)
     lens, counts, scratch = ints[:rows], ints[rows:rows + 3], ints.data_ptr() + 4 * (rows + 3)
-    with torch.cuda.device(device):
+    with _device_guard(device):
         _lib.check(_lib.load().pa_fork_sequences(
             ptr, layer_stride, layers, page_stride, page_bytes, pages, block_tables.data_ptr(),
             _row_stride(block_tables), width, seq_lens.data_ptr(), parents.data_ptr(), rows,
             kv_pool.size(-2), ref_counts.data_ptr(), out.data_ptr(), _row_stride(out),
-            lens.data_ptr(), counts.data_ptr(), scratch, _stream(device)), "fork_sequences")
+            lens.data_ptr(), counts.data_ptr(), scratch, _stream()), "fork_sequences")
         _after("fork_sequences")
     return out, lens, counts
 
@@ -180,11 +176,11 @@ def compact_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: t
     remap = torch.empty(pages, dtype=torch.int32, device=device)
     counts = torch.empty(3, dtype=torch.int32, device=device)
     scratch = torch.empty(pages + 2, dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
+    with _device_guard(device):
         _lib.check(_lib.load().pa_compact_pages(
             ptr, layer_stride, layers, page_stride, page_bytes, pages, block_tables.data_ptr(),
             _row_stride(block_tables), block_tables.size(1), seq_lens.data_ptr(),
             seq_lens.numel(), kv_pool.size(-2), ref_counts.data_ptr(), remap.data_ptr(),
-            counts.data_ptr(), scratch.data_ptr(), _stream(device)), "compact_pages")
+            counts.data_ptr(), scratch.data_ptr(), _stream()), "compact_pages")
         _after("compact_pages")
     return remap, counts

@@ -29,7 +29,7 @@ def beam(fi):
 def plain_select(logits, scores, n):
     """(scores, parents, tokens, tolerance) as numpy arrays."""
     x = logits.cpu().double().numpy()
-    x = np.where(np.isnan(x), -np.inf, np.minimum(x, float(np.finfo(np.float32).max)))
+    x = np.where(np.isnan(x), -np.inf, np.minimum(x, torch.finfo(logits.dtype).max))
     c = scores.cpu().double().numpy()
     batch, beams, vocab = x.shape
     out = [np.zeros((batch, n)) for _ in range(4)]
