@@ -22,6 +22,7 @@ _DTYPES = {torch.float16: _lib.PA_DTYPE_F16, torch.bfloat16: _lib.PA_DTYPE_BF16,
 MAX_CANDIDATES = 32
 MAX_BEAMS = 256
 MAX_VOCAB = 2 ** 24
+MAX_BATCH = 65535
 
 
 @functools.lru_cache(maxsize=256)
@@ -55,9 +56,9 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
     n = int(num_candidates)
     if beams == 0 or vocab == 0 or not 1 <= n <= beams * vocab:
         raise ValueError("num_candidates must be in [1, beams * vocab]")
-    if n > MAX_CANDIDATES or beams > MAX_BEAMS or vocab > MAX_VOCAB:
+    if n > MAX_CANDIDATES or beams > MAX_BEAMS or vocab > MAX_VOCAB or batch > MAX_BATCH:
         raise NotImplementedError(f"at most {MAX_CANDIDATES} candidates of {MAX_BEAMS} beams and "
-                                  f"{MAX_VOCAB} tokens")
+                                  f"{MAX_VOCAB} tokens, {MAX_BATCH} requests")
     if vocab > 1 and logits.stride(2) != 1:
         raise ValueError("the vocabulary dimension of logits must be contiguous")
     if scores.size(1) > 1 and scores.stride(1) != 1:

@@ -220,7 +220,7 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p, int bytes) {
 // own: maxima and comparisons pass over it, and a thread whose sum comes out
 // NaN cleans its logits and adds them up again.
 template <typename T, int VPT>
-__global__ void __launch_bounds__(kBeamThreads, 3) beam_chunk_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamParams p) {
   using W = BeamWord<T>;
   constexpr int N = 16 / sizeof(T);
   constexpr int CH = kBeamThreads * N * VPT;
@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_chunk_kernel(const BeamP
   griddep_wait();
   griddep_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
-  const int b = row / p.beams, w = row - b * p.beams;
+  const int chunk = blockIdx.x, w = blockIdx.y, b = blockIdx.z;
+  const int64_t part = (static_cast<int64_t>(b) * p.beams + w) * p.chunks + chunk;
   const T* x = static_cast<const T*>(p.logits) + b * p.stride_b + w * p.stride_w;
   const int base = chunk * CH, K = p.k;
   if (tid == 0) s_n = s_nwho = 0;
@@ -341,17 +341,25 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_chunk_kernel(const BeamP
     return base + (i * kBeamThreads + tid) * N + q * W::N + e;
   };
   const int nwho = s_nwho;
-  if (!dead && lane < VPT * 4) {
+  if (!dead) {
     for (int k = wid; k < nwho; k += kBeamWarps) {
-      const int at = base + ((lane >> 2) * kBeamThreads + s_who[k]) * N + (lane & 3) * W::N;
 #pragma unroll
-      for (int e = 0; e < W::N; ++e) {
-        if (at + e >= p.vocab) continue;
-        const float raw = static_cast<float>(__ldg(x + at + e));
-        const float f = fminf(raw, W::kMost) + 0.f;
-        if (raw == raw && order_bits(f) >= least) {
-          const int n = atomicAdd(&s_n, 1);
-          if (n < kBeamCap) s_cand[n] = beam_key(f, at + e);
+      for (int word = lane; word < VPT * 4; word += 32) {
+        const int at = base + ((word >> 2) * kBeamThreads + s_who[k]) * N + (word & 3) * W::N;
+        if (whole) {  // aligned: both of a word at once; mostly neither passes
+          const uint32_t v2 = W::clean(__ldg(reinterpret_cast<const uint32_t*>(x + at)));
+          const float f = W::N == 2 ? fmaxf(W::at(v2, 0), W::at(v2, 1)) : W::at(v2, 0);
+          if (order_bits(f + 0.f) < least) continue;
+        }
+#pragma unroll
+        for (int e = 0; e < W::N; ++e) {
+          if (at + e >= p.vocab) continue;
+          const float raw = static_cast<float>(__ldg(x + at + e));
+          const float f = fminf(raw, W::kMost) + 0.f;
+          if (raw == raw && order_bits(f) >= least) {
+            const int n = atomicAdd(&s_n, 1);
+            if (n < kBeamCap) s_cand[n] = beam_key(f, at + e);
+          }
         }
       }
     }
@@ -361,10 +369,10 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_chunk_kernel(const BeamP
     double total = 0.0;
 #pragma unroll
     for (int k = 0; k < kBeamWarps; ++k) total += s_sum[k];
-    p.part_off[blockIdx.x] = huge ? m * 1.4426950408889634 : off;
-    p.part_sum[blockIdx.x] = total;
+    p.part_off[part] = huge ? m * 1.4426950408889634 : off;
+    p.part_sum[part] = total;
   }
-  uint64_t* out = p.part_key + static_cast<int64_t>(blockIdx.x) * K;
+  uint64_t* out = p.part_key + part * K;
   int n = s_n;
   if (n > kBeamCap || least <= order_bits(-INFINITY)) {
     // many equal the threshold (or NaN counts as -inf, which nothing above
@@ -455,10 +463,13 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_chunk_kernel(const BeamP
 }
 
 // One request: the rows' sums, then the K best of its chunks' candidates.
+// Latency: a handful of dependent L2 reads and two barriers.
+constexpr int kBeamHeld = 4;  // candidates a thread keeps between the passes
+
 __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const BeamParams p) {
   extern __shared__ uint8_t beam_smem[];
-  float* s_lse = reinterpret_cast<float*>(beam_smem);  // [beams]
-  double* s_base = reinterpret_cast<double*>(beam_smem + ((p.beams * 4 + 7) & ~7));  // [beams]
+  double* s_base = reinterpret_cast<double*>(beam_smem);  // [beams]: score, -inf: no continuation
+  double* s_lse = s_base + p.beams;                       // [beams]
   __shared__ alignas(16) uint32_t s_four[32];
   __shared__ JoinKey s_key[kBeamWarps];
   __shared__ JoinKey s_cand[kBeamCap];
@@ -467,59 +478,104 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const BeamParam
   griddep_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int b = blockIdx.x, K = p.k, C = p.chunks;
+  const int lists = p.beams * C, total = lists * K;
+  const uint64_t* keys = p.part_key + static_cast<int64_t>(b) * total;
+  // candidate i of the request: entry i / lists of list i % lists; list l is
+  // chunk l / beams of beam l % beams, so that every warp starts on all beams
+  // (the best ones hold most of the winners) and on their lists' best entries
+  const int e_step = kBeamThreads / lists, l_step = kBeamThreads - e_step * lists;
+  const int e0 = tid / lists, l0 = tid - e0 * lists;
+  const float inv = 1.f / p.beams;
+  auto beam_of = [&](int l) {  // l % beams, l < 2^22
+    return l - __float2int_rd((l + 0.5f) * inv) * p.beams;
+  };
+  auto read = [&](int e, int l) {
+    const int c = __float2int_rd((l + 0.5f) * inv), w = l - c * p.beams;
+    return __ldcg(keys + (static_cast<int64_t>(w) * C + c) * K + e);
+  };
+  // the first ones' keys are read while the sums are joined
+  uint64_t held[kBeamHeld];
+  {
+    int e = e0, l = l0;
+#pragma unroll
+    for (int i = 0; i < kBeamHeld; ++i) {
+      held[i] = tid + i * kBeamThreads < total ? read(e, l) : 0;
+      e += e_step;
+      l += l_step;
+      if (l >= lists) l -= lists, ++e;
+    }
+  }
   if (tid == 0) s_n = 0;
   for (int w = wid; w < p.beams; w += kBeamWarps) {
     const int64_t at = (static_cast<int64_t>(b) * p.beams + w) * C;
-    double m = -INFINITY;
-    for (int c = lane; c < C; c += 32) m = fmax(m, __ldcg(p.part_off + at + c));
+    const float c = p.scores[b * p.score_stride + w];
+    double m = -INFINITY, sum = 0.0;
+    for (int c0 = 0; c0 < C; c0 += 32) {  // (one round up to 32 chunks)
+      const bool in = c0 + lane < C;
+      const double mc = in ? __ldcg(p.part_off + at + c0 + lane) : -INFINITY;
+      const double sc = in ? __ldcg(p.part_sum + at + c0 + lane) : 0.0;
+      double top = mc;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, off));
-    double sum = 0.0;
-    for (int c = lane; c < C; c += 32) {
-      const double mc = __ldcg(p.part_off + at + c);
-      if (mc != -INFINITY) sum += exp2(mc - m) * __ldcg(p.part_sum + at + c);
+      for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = fmax(top, m);
+      if (top == -INFINITY) continue;
+      // (a weight's fp32 exponential is as exact as the summands are)
+      double add = mc == -INFINITY ? 0.0 : ex2(static_cast<float>(mc - top)) * sc;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+      sum = (m == -INFINITY ? 0.0 : sum * ex2(static_cast<float>(m - top))) + add;
+      m = top;
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (lane == 0) {
-      const float c = p.scores[b * p.score_stride + w];
       const bool dead = m == -INFINITY || !(c > -INFINITY);  // continues nothing
-      s_lse[w] = dead ? 0.f : static_cast<float>((m + log2(sum)) * 0.6931471805599453);
+      // log2(sum): the exponent, and fp32's logarithm of the mantissa in [1, 2)
+      int ex = 0;
+      const float mant = 2.f * static_cast<float>(frexp(sum, &ex));
+      const double lse2 = m + (ex - 1) + static_cast<double>(log2f(mant));
+      s_lse[w] = dead ? 0.0 : static_cast<float>(lse2 * 0.6931471805599453);
       s_base[w] = dead ? -INFINITY : static_cast<double>(fminf(c, 3.402823466e38f));
     }
   }
   __syncthreads();
-  // candidate i of the request: entry i / lists of list i % lists (a list is
-  // a row's chunk), so that a warp's threads start on different lists
-  const int lists = p.beams * C, total = lists * K;
-  const uint64_t* keys = p.part_key + static_cast<int64_t>(b) * total;
-  auto candidate = [&](int i) {
-    const int e = i / lists, l = i - e * lists;
-    const uint64_t key = __ldcg(keys + static_cast<int64_t>(l) * K + e);
+  auto candidate = [&](uint64_t key, int l) {
     if (key == 0) return JoinKey{0, 0};
-    const int w = l / C;
+    const int w = beam_of(l);
     const float x = order_value(static_cast<uint32_t>(key >> 32));
-    const double s = x == -INFINITY ? -INFINITY
-                                    : s_base[w] + (static_cast<double>(x) - s_lse[w]);
+    const double s = x == -INFINITY ? -INFINITY : s_base[w] + (x - s_lse[w]);
     const uint32_t token = 0xffffffffu - static_cast<uint32_t>(key);
     return JoinKey{order_bits64(s), (static_cast<uint64_t>(255 - w) << 56) |
                                         ((key >> 32) << 24) | (0xffffffu - token)};
   };
+  // f(candidate) for every candidate of this thread
+  auto each = [&](auto f) {
+    int e = e0, l = l0;
+#pragma unroll
+    for (int i = 0; i < kBeamHeld; ++i) {
+      f(candidate(held[i], l));
+      e += e_step;
+      l += l_step;
+      if (l >= lists) l -= lists, ++e;
+    }
+    for (int i = tid + kBeamHeld * kBeamThreads; i < total; i += kBeamThreads) {
+      f(candidate(read(e, l), l));
+      e += e_step;
+      l += l_step;
+      if (l >= lists) l -= lists, ++e;
+    }
+  };
   uint64_t best = 0;
-  for (int i = tid; i < total; i += kBeamThreads) best = max(best, candidate(i).score);
+  each([&](const JoinKey& c) { best = max(best, c.score); });
   // (the upper half of the score's bits is threshold enough)
   uint32_t top;
   const uint32_t least = block_threshold(static_cast<uint32_t>(best >> 32), K, s_four, lane, wid,
                                          &top);
-  if (best != 0 && best >> 32 >= least) {
-    for (int i = tid; i < total; i += kBeamThreads) {
-      const JoinKey c = candidate(i);
+  if (best != 0 && best >> 32 >= least)
+    each([&](const JoinKey& c) {
       if (c.score != 0 && c.score >> 32 >= least) {
         const int at = atomicAdd(&s_n, 1);
         if (at < kBeamCap) s_cand[at] = c;
       }
-    }
-  }
+    });
   __syncthreads();
   auto put = [&](int k, const JoinKey& c) {
     p.out_scores[b * K + k] = static_cast<float>(order_value64(c.score));
@@ -539,10 +595,9 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const BeamParam
   JoinKey last{~0ULL, ~0ULL};
   for (int k = 0; k < K; ++k) {
     JoinKey next{0, 0};
-    for (int i = tid; i < total; i += kBeamThreads) {
-      const JoinKey c = candidate(i);
+    each([&](const JoinKey& c) {
       if (last > c && c > next) next = c;
-    }
+    });
     last = block_max<JoinKey>(next, s_key, lane, wid);
     if (tid == 0) put(k, last);
   }
