@@ -1255,10 +1255,15 @@ int pa_window_decode_plan(const int32_t* kv_indptr, const int32_t* kv_indices,
                               decode_ws_bytes(sh, batch_size, num_kv_heads, head_dim));
   if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
   const int copiers = std::min(batch_size, sh.ctas - 1);
+  // Windows make short streams, so few requests leave most SMs idle unless
+  // they are cut finer than whole contexts are: runs of 2 pages and up to 32
+  // pieces a segment (one request over 4096 keys: 27 us, 50 with the full
+  // plan's 4 and 8; four requests over 1024: 22 and 28; 64 or more: no change).
   return launch_chain(window_decode_plan_kernel, dim3(1 + copiers), dim3(kWindowPlanThreads), 0,
                       static_cast<cudaStream_t>(stream), kv_indptr, kv_last_page_len, kv_indices,
                       num_kv_indices, batch_size, num_kv_heads, num_qo_heads, head_dim, page_size,
-                      window_left, num_sink_tokens, sh.units, sh.g.hb, /*min_per_group=*/4,
+                      window_left, num_sink_tokens, sh.units, sh.g.hb, /*min_per_group=*/2,
+                      /*max_pieces=*/32,
                       static_cast<uint8_t*>(workspace), L);
 }
 

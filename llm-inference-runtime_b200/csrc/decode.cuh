@@ -99,7 +99,7 @@ __device__ void decode_plan_block(const Indptr kv_indptr,
                                   int hq, int head_dim, int page_size, int64_t num_indices,
                                   int num_groups, int hb, int min_per_group,
                                   uint8_t* __restrict__ ws, int32_t magic = kDecodeMagic,
-                                  bool bad_table = false) {
+                                  bool bad_table = false, int max_pieces = 8) {
   const DecodeWsLayout L = decode_ws_layout(num_groups, batch, hkv, head_dim, hb);
   DecodePlanHeader* hdr = reinterpret_cast<DecodePlanHeader*>(ws + L.hdr);
   int4* unit_start = reinterpret_cast<int4*>(ws + L.unit_start);
@@ -136,13 +136,13 @@ __device__ void decode_plan_block(const Indptr kv_indptr,
   const int total = err ? 0 : static_cast<int>(total_ll);
   int q = (total + num_groups - 1) / num_groups;
   q = max(q, min_per_group);
-  // At most ~8 pieces per (request, head block) segment on average: the
+  // At most ~max_pieces pieces per (request, head block) segment on average: the
   // warp that merges a split segment reads its pieces two per L2 round
   // trip, so short runs over long segments (32 requests of 256-2048 tokens
   // over 444 groups: 6 pages per run, 12 pieces) cost more in merges than
   // the extra groups gain.
   const int segs = nhb * (batch - s_empty);
-  if (!err && segs > 0) q = max(q, (total + 8 * segs - 1) / (8 * segs));
+  if (!err && segs > 0) q = max(q, (total + max_pieces * segs - 1) / (max_pieces * segs));
   for (int w = threadIdx.x; w < num_groups; w += blockDim.x) {
     const long long s0 = static_cast<long long>(w) * q;
     int4 st = make_int4(0, 0, 0, 0);
@@ -223,29 +223,28 @@ struct MergeSeg {
 // kItems granules per lane at a time; the LSEs and partial rows of kBatch
 // pieces of every granule of both segments are loaded together (online
 // max), so merging both segments costs one L2 round trip per kBatch pieces
-// rather than one per granule, piece or segment.
-template <typename T, int D>
+// rather than one per granule, piece or segment. kSegs = 1: `sa` alone.
+template <typename T, int D, int kSegs = 2, int kBatch = 2>
 __device__ __noinline__ void merge_segments(const float* part_lse, const float* part_o, T* out,
                                             float* lse, int* counter, int G, int hq, int hkv,
                                             int Q, int HB, int hh, MergeSeg sa, MergeSeg sb,
                                             int nseg, int lane) {
   constexpr int C4 = D / 4;
   constexpr int kItems = 4;
-  constexpr int kBatch = 2;
   const int n_items = G * C4;
   const MergeSeg seg[2] = {sa, sb};
-  int u0[2], np[2];
+  int u0[kSegs], np[kSegs];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
+  for (int s = 0; s < kSegs; ++s) {
     u0[s] = seg[s].seg_start / Q;
     np[s] = s < nseg ? (seg[s].seg_start + seg[s].seg_len - 1) / Q - u0[s] + 1 : 0;
   }
-  const int np_max = max(np[0], np[1]);
+  const int np_max = max(np[0], np[kSegs - 1]);
   for (int it0 = 0; it0 < n_items; it0 += 32 * kItems) {
-    float m[2][kItems], w[2][kItems];
-    float4 acc[2][kItems];
+    float m[kSegs][kItems], w[kSegs][kItems];
+    float4 acc[kSegs][kItems];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < kSegs; ++s)
 #pragma unroll
       for (int j = 0; j < kItems; ++j) {
         m[s][j] = -INFINITY;
@@ -253,10 +252,10 @@ __device__ __noinline__ void merge_segments(const float* part_lse, const float* 
         acc[s][j] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
     for (int ub = 0; ub < np_max; ub += kBatch) {
-      float lb[2][kItems][kBatch];
-      float4 vb[2][kItems][kBatch];
+      float lb[kSegs][kItems][kBatch];
+      float4 vb[kSegs][kItems][kBatch];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < kSegs; ++s)
 #pragma unroll
         for (int j = 0; j < kItems; ++j) {
           const int it = it0 + j * 32 + lane;
@@ -276,7 +275,7 @@ __device__ __noinline__ void merge_segments(const float* part_lse, const float* 
           }
         }
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < kSegs; ++s)
 #pragma unroll
         for (int j = 0; j < kItems; ++j)
 #pragma unroll
@@ -293,7 +292,7 @@ __device__ __noinline__ void merge_segments(const float* part_lse, const float* 
           }
     }
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kSegs; ++s) {
       if (s >= nseg) break;
       T* ob = out + (static_cast<size_t>(seg[s].b) * hq + seg[s].head * G) * D;
 #pragma unroll
@@ -818,8 +817,16 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
       const MergeSeg s0{pend_b[0], pend_head[0], pend_seg[0], pend_len[0]};
       const MergeSeg s1{pend_b[1], pend_head[1], pend_seg[1], pend_len[1]};
       __threadfence();
-      merge_segments<T, D>(p.part_lse, p.part_o, out, p.lse, p.counter, G, hq, hkv, Q, HB, hh,
-                           last0 ? s0 : s1, s1, last0 && last1 ? 2 : 1, lane);
+      if (kWindow && !(last0 && last1))
+        // a plan of few requests cuts them into up to 32 pieces: more of one
+        // segment's pieces in flight (with 2 at a time a window of 4096 keys
+        // of one request takes 29.0 us, with 6 27.4)
+        merge_segments<T, D, 1, D == 128 ? 6 : 4>(p.part_lse, p.part_o, out, p.lse, p.counter, G,
+                                                  hq, hkv, Q, HB, hh, last0 ? s0 : s1, s1, 1,
+                                                  lane);
+      else
+        merge_segments<T, D>(p.part_lse, p.part_o, out, p.lse, p.counter, G, hq, hkv, Q, HB, hh,
+                             last0 ? s0 : s1, s1, last0 && last1 ? 2 : 1, lane);
     }
   }
 }

@@ -108,11 +108,17 @@ __device__ __forceinline__ WindowRow window_row(const int32_t* indptr, const int
   return r;
 }
 
-// Reads the indptr that this CTA wrote earlier in the launch (past the
-// read-only path, which may hold older bytes).
+// The indptr that this CTA has just made: its first kWindowHeld entries in
+// shared memory, the others read past the read-only path (which may hold
+// older bytes).
+constexpr int kWindowHeld = 2048;
+
 struct FreshIndptr {
-  const int32_t* p;
-  __device__ __forceinline__ int operator[](int i) const { return __ldcg(p + i); }
+  const int32_t* held;
+  const int32_t* all;
+  __device__ __forceinline__ int operator[](int i) const {
+    return i < kWindowHeld ? held[i] : __ldcg(all + i);
+  }
 };
 
 constexpr int kWindowPlanThreads = 1024;
@@ -126,13 +132,14 @@ __global__ void __launch_bounds__(kWindowPlanThreads)
                               const int32_t* __restrict__ last_len,
                               const int32_t* __restrict__ kv_indices, int64_t num_indices,
                               int batch, int hkv, int hq, int head_dim, int page_size, int window,
-                              int sinks, int num_groups, int hb, int min_per_group,
+                              int sinks, int num_groups, int hb, int min_per_group, int max_pieces,
                               uint8_t* __restrict__ ws, WindowDecodeWsLayout L) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ int s_warp[32];
   __shared__ int s_carry;
   __shared__ int s_bad;
+  __shared__ int32_t s_held[kWindowHeld];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   if (blockIdx.x == 0) {
     int32_t* out_indptr = reinterpret_cast<int32_t*>(ws + L.indptr);
@@ -140,7 +147,7 @@ __global__ void __launch_bounds__(kWindowPlanThreads)
     if (tid == 0) {
       s_carry = 0;
       s_bad = __ldg(kv_indptr) != 0;
-      out_indptr[0] = 0;
+      out_indptr[0] = s_held[0] = 0;
     }
     __syncthreads();
     for (int b0 = 0; b0 < batch; b0 += kWindowPlanThreads) {
@@ -168,16 +175,18 @@ __global__ void __launch_bounds__(kWindowPlanThreads)
       __syncthreads();
       const int carry = s_carry;
       if (b < batch) {
-        out_indptr[b + 1] = carry + (wid > 0 ? s_warp[wid - 1] : 0) + incl;
+        const int end = carry + (wid > 0 ? s_warp[wid - 1] : 0) + incl;
+        out_indptr[b + 1] = end;
+        if (b + 1 < kWindowHeld) s_held[b + 1] = end;
         out_window[b] = make_int4(r.span.hole_lo, r.span.hole_hi, r.span.sink_pages, r.span.shift);
       }
       __syncthreads();
       if (tid == 0) s_carry = carry + s_warp[31];
       __syncthreads();
     }
-    decode_plan_block(FreshIndptr{out_indptr}, last_len, batch, hkv, hq, head_dim, page_size,
+    decode_plan_block(FreshIndptr{s_held, out_indptr}, last_len, batch, hkv, hq, head_dim, page_size,
                       L.capacity, num_groups, hb, min_per_group, ws + L.decode,
-                      kWindowDecodeMagic, s_bad != 0);
+                      kWindowDecodeMagic, s_bad != 0, max_pieces);
     return;
   }
   int32_t* out_indices = reinterpret_cast<int32_t*>(ws + L.indices);

@@ -172,14 +172,19 @@ def test_decode_batch_larger_than_the_grid(fi, window, sinks):
     pr.check(out, lse)
 
 
-def test_decode_equals_the_full_wrapper_when_all_is_visible(fi):
+def test_decode_agrees_with_the_full_wrapper_when_all_is_visible(fi):
+    """The window plan cuts segments into other pieces than the full one, and
+    each piece rounds its probabilities against its own maximum: each of the
+    two is within the tolerance, so they are within twice that of each other
+    (not bit-identical, as they would be on one partition)."""
     pr = _decode_problem(MIXED, 32, 4, 64, HUGE, 0, seed=3)
     pool, q = pr.device_pool(), pr.q.to(DEV)
     got, glse = _decode_wrapper(fi, pr).run(q, pool, return_lse=True)
     w = fi.BatchDecodeWithPagedKVCacheWrapper(_ws(), "HND")
     w.plan(_t(pr.indptr), _t(pr.indices), _t(pr.last), 32, 4, 64, P, q_data_type=pr.dtype)
     out, lse = w.run(q, pool, return_lse=True)
-    assert torch.equal(got, out) and torch.equal(glse, lse)
+    pr.check(got, glse)
+    pr.check(out, lse)
 
 
 @pytest.mark.parametrize("hq,hkv,d,layout,dtype", [(8, 2, 64, "HND", torch.bfloat16),
