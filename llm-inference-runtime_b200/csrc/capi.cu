@@ -625,7 +625,7 @@ int launch_copy_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers
   c.count = count;
   const int64_t units = most * num_layers * ((page_bytes + kCopySlice - 1) / kCopySlice);
   const int64_t sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min(units, sms)));
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min(units, sms * kCopyCtas)));
   return launch_chain(copy_pages_kernel, dim3(grid), dim3(32), kCopySmem, stream, c);
 }
 

@@ -20,13 +20,16 @@ namespace pa {
 
 // ------------------------------------------------------------ bulk page copy
 // Copies (pair, layer) blocks of page_bytes: pages src[i] -> dst[i] for
-// i < *count, every layer. Bound by HBM (each byte read and written once):
-// one thread per CTA runs a ring of kCopyStages slices of kCopySlice bytes
-// through shared memory with bulk copies in both directions, so no byte
-// passes through registers and each SM has up to 128 KB in flight.
+// i < *count, every layer. Bound by HBM (each byte read and written once): a
+// warp per CTA runs a ring of kCopyStages slices of kCopySlice bytes through
+// shared memory with bulk copies in both directions, so no byte passes
+// through registers. One thread issues them; the addresses of 32 units at a
+// time are worked out lane by lane.
 constexpr int kCopySlice = 16 * 1024;
-constexpr int kCopyStages = 8;
+constexpr int kCopyStages = 6;
+constexpr int kCopyCtas = 2;  // per SM
 constexpr int kCopySmem = kCopySlice * kCopyStages + 128;
+static_assert(kCopyStages < 32, "a load is at most one batch of units ahead of its store");
 
 struct CopyParams {
   uint8_t* pool;
@@ -37,7 +40,7 @@ struct CopyParams {
   const int32_t* count;  // device word
 };
 
-__global__ void __launch_bounds__(32, 1) copy_pages_kernel(const CopyParams p) {
+__global__ void __launch_bounds__(32, kCopyCtas) copy_pages_kernel(const CopyParams p) {
   extern __shared__ uint8_t copy_smem[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(copy_smem) + 127) &
                                              ~uintptr_t(127));
@@ -55,52 +58,84 @@ __global__ void __launch_bounds__(32, 1) copy_pages_kernel(const CopyParams p) {
   // this CTA's units: blockIdx.x + i * gridDim.x, i < mine
   const int64_t mine =
       total > blockIdx.x ? (total - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
-  if (lane != 0) return;
-  auto unit = [&](int64_t i, uint8_t** from, uint8_t** to, uint32_t* bytes) {
-    const int64_t u = blockIdx.x + i * gridDim.x;
-    const int64_t pair = u / per_pair, rem = u - pair * per_pair;
-    const int64_t layer = rem / slices, sl = rem - layer * slices;
-    const int64_t off = layer * p.layer_stride + sl * kCopySlice;
-    const int64_t left = p.page_bytes - sl * kCopySlice;
-    *bytes = static_cast<uint32_t>(left < kCopySlice ? left : kCopySlice);
-    *from = p.pool + off + __ldcg(p.src + pair) * p.page_stride;
-    *to = p.pool + off + __ldcg(p.dst + pair) * p.page_stride;
-  };
-  auto load = [&](int64_t i) {
-    uint8_t *from, *to;
+  struct Unit {
+    uint64_t from, to;
     uint32_t bytes;
-    unit(i, &from, &to, &bytes);
-    const int st = static_cast<int>(i % kCopyStages);
-    mbar_arrive_expect_tx(&full[st], bytes);
-    bulk_load(ring + st * kCopySlice, from, bytes, &full[st]);
   };
-  const int64_t ahead = mine < kCopyStages ? mine : kCopyStages;
-  for (int64_t i = 0; i < ahead; ++i) load(i);
-  int64_t loaded = ahead;
+  auto batch = [&](int64_t first) {  // lane l: unit first + l of this CTA
+    Unit n{0, 0, 0};
+    if (first + lane < mine) {
+      const int64_t u = blockIdx.x + (first + lane) * gridDim.x;
+      const int64_t pair = u / per_pair, rem = u - pair * per_pair;
+      const int64_t layer = rem / slices, sl = rem - layer * slices;
+      const uint64_t at =
+          reinterpret_cast<uint64_t>(p.pool) + layer * p.layer_stride + sl * kCopySlice;
+      const int64_t left = p.page_bytes - sl * kCopySlice;
+      n.bytes = static_cast<uint32_t>(left < kCopySlice ? left : kCopySlice);
+      n.from = at + __ldcg(p.src + pair) * p.page_stride;
+      n.to = at + __ldcg(p.dst + pair) * p.page_stride;
+    }
+    return n;
+  };
+  Unit a = batch(0), b = batch(32);  // the current 32 units and the next
+  int64_t a0 = 0;
+  auto load = [&](int64_t i, int stage) {  // every lane calls it
+    const int l = static_cast<int>(i - a0);
+    const uint64_t from = __shfl_sync(0xffffffffu, l < 32 ? a.from : b.from, l & 31);
+    const uint32_t bytes = __shfl_sync(0xffffffffu, l < 32 ? a.bytes : b.bytes, l & 31);
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&full[stage], bytes);
+      bulk_load(ring + stage * kCopySlice, reinterpret_cast<const void*>(from), bytes,
+                &full[stage]);
+    }
+  };
+  int64_t loaded = 0;
+  for (; loaded < mine && loaded < kCopyStages; ++loaded) load(loaded, static_cast<int>(loaded));
+  int stage = 0;
+  uint32_t phase = 0;
+  bool failed = false;
   for (int64_t i = 0; i < mine; ++i) {
-    const int st = static_cast<int>(i % kCopyStages);
-    if (!mbar_wait(&full[st], static_cast<uint32_t>(i / kCopyStages) & 1)) {
-      set_status(PA_ERR_TIMEOUT);
-      // the other loads in flight land (or time out too) before this CTA ends
-      for (int64_t k = i + 1; k < loaded; ++k)
-        mbar_wait(&full[k % kCopyStages], static_cast<uint32_t>(k / kCopyStages) & 1);
+    if (i - a0 == 32) {
+      a0 += 32;
+      a = b;
+      b = batch(a0 + 32);
+    }
+    const int l = static_cast<int>(i - a0);
+    const uint64_t to = __shfl_sync(0xffffffffu, a.to, l);
+    const uint32_t bytes = __shfl_sync(0xffffffffu, a.bytes, l);
+    if (!mbar_wait_warp(&full[stage], phase)) {
+      failed = true;
       break;
     }
-    uint8_t *from, *to;
-    uint32_t bytes;
-    unit(i, &from, &to, &bytes);
-    bulk_store(to, ring + st * kCopySlice, bytes);
-    bulk_commit();
+    if (lane == 0) {
+      bulk_store(reinterpret_cast<void*>(to), ring + stage * kCopySlice, bytes);
+      bulk_commit();
+    }
     // refill the stage of unit i - 1, whose store has had a unit's time to
     // read it
-    const int64_t next = i - 1 + kCopyStages;
-    if (i >= 1 && next < mine) {
-      bulk_wait_read_but<1>();
-      load(next);
-      loaded = next + 1;
+    if (i >= 1 && loaded < mine) {
+      if (lane == 0) bulk_wait_read_but<1>();
+      __syncwarp();
+      load(loaded, stage == 0 ? kCopyStages - 1 : stage - 1);
+      ++loaded;
+    }
+    if (++stage == kCopyStages) {
+      stage = 0;
+      phase ^= 1;
     }
   }
-  bulk_wait_all();
+  if (failed) {
+    if (lane == 0) set_status(PA_ERR_TIMEOUT);
+    // the other loads in flight land (or time out too) before this CTA ends
+    for (int s = 1; s < kCopyStages; ++s) {
+      if (++stage == kCopyStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      mbar_wait_warp(&full[stage], phase);
+    }
+  }
+  if (lane == 0) bulk_wait_all();
 }
 
 // ------------------------------------------------------------ giving pages back
