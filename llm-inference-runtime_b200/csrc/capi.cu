@@ -265,9 +265,8 @@ int launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorM
   // persistent: one CTA per SM at most, each taking items until none is left
   const int sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
   grid = std::min<int64_t>(grid, sms);
-  prefill_kernel<T, D, kWindow>
-      <<<static_cast<unsigned>(grid), kPfThreads, smem, stream>>>(qm, km, vm, om, prm);
-  return launch_status();
+  return launch_chain(prefill_kernel<T, D, kWindow>, dim3(static_cast<unsigned>(grid)),
+                      dim3(kPfThreads), smem, stream, qm, km, vm, om, prm);
 }
 
 template <bool kWindow>
@@ -1399,11 +1398,11 @@ int prefill_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
   const int64_t max_items = prefill_max_items(batch_size, total_qo, num_kv_heads, span);
   if (prefill_ws_layout(max_items).total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
   // one thread per cost bucket (the plan's scan relies on it)
-  prefill_plan_kernel<<<1, kPfCostBuckets, 0, static_cast<cudaStream_t>(stream)>>>(
-      qo_indptr, kv_indptr, kv_last_page_len, batch_size, total_qo, num_kv_indices, num_qo_heads,
-      num_kv_heads, head_dim, page_size, span, max_items, window_left, num_sink_tokens,
-      static_cast<uint8_t*>(workspace));
-  return launch_status();
+  return launch_chain(prefill_plan_kernel, dim3(1), dim3(kPfCostBuckets), 0,
+                      static_cast<cudaStream_t>(stream), qo_indptr, kv_indptr, kv_last_page_len,
+                      batch_size, total_qo, num_kv_indices, num_qo_heads, num_kv_heads, head_dim,
+                      page_size, span, max_items, window_left, num_sink_tokens,
+                      static_cast<uint8_t*>(workspace));
 }
 
 int prefill_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_kv_cache* cache,

@@ -358,55 +358,65 @@ __global__ void __launch_bounds__(kForkThreads) fork_rows_kernel(const ForkSeqPa
   if (tid == 0) p.out_lens[r] = f.ok ? f.len : 0;
 }
 
+// One CTA; bound by its chain of dependent L2 reads, so the first 1024 rows
+// and the first kScanThreads * kPerThread counts stay in registers, and the
+// free pages' numbers in shared memory.
 __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeqParams p) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ int s_warp[32];
+  __shared__ int s_avail[kScanThreads];
   const int tid = threadIdx.x;
   const int rounds = (p.rows + kScanThreads - 1) / kScanThreads;
+  const ForkRow none{0, 0, 0, -1, false};
+  const ForkRow first = tid < p.rows ? fork_row(p, tid) : none;
+  int state0 = 0;  // state of row `tid`; later rows' in p.state
+  auto row = [&](int k) {
+    const int r = k * kScanThreads + tid;
+    return k == 0 ? first : r < p.rows ? fork_row(p, r) : none;
+  };
+  auto get = [&](int k) {
+    const int r = k * kScanThreads + tid;
+    return k == 0 ? state0 : r < p.rows ? p.state[r] : 0;
+  };
+  auto set = [&](int k, int v) {
+    const int r = k * kScanThreads + tid;
+    if (k == 0)
+      state0 = v;
+    else if (r < p.rows)
+      p.state[r] = v;
+  };
   // Claims on unfinished pages that nobody else holds: the count (0 now)
-  // serves as the ballot, rows - r being larger for earlier rows. Rows of
-  // later rounds see a claimed page as such because claims of all rounds
-  // are settled only after every row has looked. state[r] carries the
-  // row's state between the passes.
+  // serves as the ballot, rows - r being larger for earlier rows. Every row
+  // looks before any row claims, and claims are settled before any is
+  // answered.
+  for (int k = 0; k < rounds; ++k) {
+    const ForkRow f = row(k);
+    set(k, f.last >= 0 && f.ok && __ldcg(p.refs + f.last) == 0);
+  }
+  __syncthreads();
+  for (int k = 0; k < rounds; ++k)
+    if (get(k)) atomicMax(p.refs + row(k).last, p.rows - (k * kScanThreads + tid));
+  __syncthreads();
+  for (int k = 0; k < rounds; ++k)
+    if (get(k) && __ldcg(p.refs + row(k).last) != p.rows - (k * kScanThreads + tid)) set(k, 0);
+  __syncthreads();
+  int total = 0;
   for (int k = 0; k < rounds; ++k) {
     const int r = k * kScanThreads + tid;
-    if (r < p.rows) {
-      const ForkRow f = fork_row(p, r);
-      p.state[r] = f.last >= 0 && f.ok && __ldcg(p.refs + f.last) == 0;
+    const ForkRow f = row(k);
+    const bool keep = get(k) != 0;
+    if (keep) {
+      p.refs[f.last] = 1;
+      p.out_tables[r * p.out_stride + f.full] = f.last;
     }
-  }
-  __syncthreads();
-  for (int k = 0; k < rounds; ++k) {
-    const int r = k * kScanThreads + tid;
-    if (r < p.rows && p.state[r]) atomicMax(p.refs + fork_row(p, r).last, p.rows - r);
-  }
-  __syncthreads();
-  for (int k = 0; k < rounds; ++k) {
-    const int r = k * kScanThreads + tid;
-    if (r < p.rows && p.state[r] && __ldcg(p.refs + fork_row(p, r).last) != p.rows - r)
-      p.state[r] = 0;
-  }
-  __syncthreads();
-  int total = 0, copies = 0;
-  for (int k = 0; k < rounds; ++k) {
-    const int r = k * kScanThreads + tid;
-    ForkRow f{0, 0, 0, -1, false};
-    bool keep = false;
-    if (r < p.rows) {
-      f = fork_row(p, r);
-      keep = p.state[r] != 0;
-      if (keep) {
-        p.refs[f.last] = 1;
-        p.out_tables[r * p.out_stride + f.full] = f.last;
-      }
-    }
-    // -1: wants nothing (keeps its page, or is not sound)
-    const bool wants = f.ok && !keep && f.full < p.width;
+    // state: rank among the rows that want a page, -1: wants none (keeps its
+    // page, or is not sound)
+    const bool wants = r < p.rows && f.ok && !keep && f.full < p.width;
     int n;
     const int at = total + block_exclusive(wants ? 1 : 0, s_warp, &n);
     total += n;
-    if (r < p.rows) p.state[r] = wants ? at : -1;
+    set(k, wants ? at : -1);
   }
   // the first `total` free pages in ascending order
   __syncthreads();
@@ -424,24 +434,28 @@ __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeq
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i)
       if (v[i] == 0) {
-        if (rank < total) p.avail[rank] = static_cast<int>(at + i);
+        if (rank < total) {
+          if (rank < kScanThreads)
+            s_avail[rank] = static_cast<int>(at + i);
+          else
+            p.avail[rank] = static_cast<int>(at + i);
+        }
         ++rank;
       }
     found += n;
   }
   found = min(found, total);
   __syncthreads();
-  int missing = 0;
+  int missing = 0, copies = 0;
   for (int k = 0; k < rounds; ++k) {
     const int r = k * kScanThreads + tid;
-    ForkRow f{0, 0, 0, -1, false};
+    const ForkRow f = row(k);
+    const int at = get(k);
     int page = -1, from = -1;
     if (r < p.rows) {
-      f = fork_row(p, r);
-      const int at = p.state[r];
       if (at >= 0) {
         if (at < found) {
-          page = __ldcg(p.avail + at);
+          page = at < kScanThreads ? s_avail[at] : __ldcg(p.avail + at);
           p.refs[page] = 1;
           from = f.last;
         }
@@ -492,10 +506,12 @@ __global__ void __launch_bounds__(kScanThreads) compact_plan_kernel(const Compac
   __shared__ int s_warp[32];
   const int tid = threadIdx.x;
   constexpr int64_t kStep = static_cast<int64_t>(kScanThreads) * kPerThread;
+  const int64_t mine = static_cast<int64_t>(tid) * kPerThread;
   int v[kPerThread];
   int live = 0;
-  for (int64_t base = 0; base < p.num_pages; base += kStep) {
-    load_counts(p.refs, base + static_cast<int64_t>(tid) * kPerThread, p.num_pages, 0, v);
+  // last step first, so that the first one's counts are at hand for the ranks
+  for (int64_t base = (p.num_pages - 1) / kStep * kStep; base >= 0; base -= kStep) {
+    load_counts(p.refs, base + mine, p.num_pages, 0, v);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) live += v[i] > 0;
   }
@@ -503,17 +519,18 @@ __global__ void __launch_bounds__(kScanThreads) compact_plan_kernel(const Compac
   block_exclusive(live, s_warp, &n_live);
   int moved = 0, holes = 0;
   for (int64_t base = 0; base < p.num_pages; base += kStep) {
-    const int64_t at = base + static_cast<int64_t>(tid) * kPerThread;
-    load_counts(p.refs, at, p.num_pages, 0, v);
+    const int64_t at = base + mine;
+    if (base > 0) load_counts(p.refs, at, p.num_pages, 0, v);
     int out = 0, in = 0;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       out += v[i] > 0 && at + i >= n_live;
       in += v[i] <= 0 && at + i < n_live;
     }
-    int n_out, n_in;
-    int o = moved + block_exclusive(out, s_warp, &n_out);
-    int h = holes + block_exclusive(in, s_warp, &n_in);
+    // both ranks in one scan: at most 16384 of each per step
+    int n_both;
+    const int both = block_exclusive(out << 16 | in, s_warp, &n_both);
+    int o = moved + (both >> 16), h = holes + (both & 0xffff);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       const int64_t page = at + i;
@@ -530,8 +547,8 @@ __global__ void __launch_bounds__(kScanThreads) compact_plan_kernel(const Compac
         p.remap[page] = -1;
       }
     }
-    moved += n_out;
-    holes += n_in;
+    moved += n_both >> 16;
+    holes += n_both & 0xffff;
   }
   __syncthreads();
   for (int k = tid; k < moved; k += kScanThreads) {

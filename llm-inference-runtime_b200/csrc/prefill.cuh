@@ -184,6 +184,8 @@ __global__ void prefill_plan_kernel(const int32_t* __restrict__ qo_indptr,
                                     int64_t total_qo, int64_t num_indices, int hq, int hkv,
                                     int head_dim, int page_size, int qt, int64_t max_items,
                                     int window, int sinks, uint8_t* __restrict__ ws) {
+  griddep_wait();
+  griddep_launch_dependents();
   const PrefillWsLayout L = prefill_ws_layout(max_items);
   PrefillPlanHeader* hdr = reinterpret_cast<PrefillPlanHeader*>(ws + L.hdr);
   int4* items = reinterpret_cast<int4*>(ws + L.items);
@@ -382,6 +384,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   PfItem* slots = reinterpret_cast<PfItem*>(smem + C::kOffSlots);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();  // launched while the plan still runs
   const PrefillPlanHeader* hdr = p.hdr;
   if (hdr->magic != kPrefillMagic || hdr->batch_size != p.batch_size ||
       hdr->num_kv_heads != p.num_kv_heads || hdr->num_qo_heads != p.num_qo_heads ||
