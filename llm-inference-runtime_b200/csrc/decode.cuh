@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
   float o[NT][4];
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   int seg_start = 0, last_len = kPage, head = 0, apos = -1;
-  int hole_lo = 0, hole_hi = 0;  // keys of the segment's stream that the window hides
+  [[maybe_unused]] int hole_lo = 0, hole_hi = 0;  // keys of the segment that the window hides
   const bool row0 = gid < G, row1 = gid + 8 < G;
   // Row of token r of this warp's head inside a panel of the stage.
   const int row_mul = p.heads_inner ? HB : 1;
@@ -526,20 +526,19 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
       l0 = l1 = 0.f;
       seg_start = NHB * cc.base + cc.hblk * cc.n;
       last_len = __ldg(p.kv_last_page_len + cc.b);
+      int4 win = make_int4(0, 0, 0, 0);
+      if constexpr (kWindow) win = __ldg(p.window + cc.b);
       if (p.append_pos != nullptr) {
         // the same rule as pa_append_paged_kv_cache: the position must fall
         // inside the request's pages
         apos = __ldg(p.append_pos + cc.b);
         if (p.append_pos_base != nullptr) apos -= __ldg(p.append_pos_base);
-        int pages = cc.n;
-        if constexpr (kWindow) pages += __ldg(&p.window[cc.b].w);
-        if (apos < 0 || apos / kPage >= pages) {
+        if (apos < 0 || apos / kPage >= (kWindow ? cc.n + win.w : cc.n)) {
           if (lane == 0) set_status(PA_ERR_DEVICE_CHECK);
           apos = -1;
         }
       }
       if constexpr (kWindow) {
-        const int4 win = __ldg(p.window + cc.b);
         hole_lo = win.x;
         hole_hi = win.y;
         if (apos >= 0 && apos / kPage >= win.z) {
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
     const uint32_t vb = kb + PANELS * panel_bytes;
     const int valid = (cc.j == cc.n - 1) ? last_len : kPage;
     // keys [h0, h1) of this page are hidden by the window
-    int h0 = 0, h1 = 0;
+    [[maybe_unused]] int h0 = 0, h1 = 0;
     if constexpr (kWindow) {
       h0 = max(hole_lo - cc.j * kPage, 0);
       h1 = max(min(hole_hi - cc.j * kPage, kPage), h0);
@@ -619,9 +618,10 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = t * 8 + 2 * tig + (e & 1);
-        bool seen = key < valid;
-        if constexpr (kWindow) seen = seen && (key < h0 || key >= h1);
-        s[t][e] = seen ? s[t][e] * p.scale_log2 : -INFINITY;
+        if constexpr (kWindow)
+          s[t][e] = key < valid && (key < h0 || key >= h1) ? s[t][e] * p.scale_log2 : -INFINITY;
+        else
+          s[t][e] = key < valid ? s[t][e] * p.scale_log2 : -INFINITY;
       }
       mx0 = fmaxf(mx0, fmaxf(s[t][0], s[t][1]));
       mx1 = fmaxf(mx1, fmaxf(s[t][2], s[t][3]));
