@@ -100,6 +100,10 @@ class PagedAttnState(metaclass=_StateMeta):
     page_size: int = 16
     dtype: Optional[torch.dtype] = None
 
+    # sliding window of every layer (None: full contexts, the reference's)
+    window_left: Optional[int] = None
+    num_sink_tokens: int = 0
+
     mode: str = "prefill"
 
 
@@ -108,17 +112,33 @@ FlashInferState = PagedAttnState
 WORKSPACE_BYTES = 128 * 1024 * 1024  # the reference's workspace size (llama.py:49-53)
 
 
-def init_flashinfer_state(*, kv_pool: torch.Tensor, page_size: int, device) -> None:
-    """Borrows the allocator's pool and builds the two wrappers ("HND")."""
+def init_flashinfer_state(*, kv_pool: torch.Tensor, page_size: int, device,
+                          window_left: Optional[int] = None, num_sink_tokens: int = 0) -> None:
+    """Borrows the allocator's pool and builds the two wrappers ("HND").
+
+    With ``window_left`` every layer attends through a sliding window of the
+    last ``window_left + 1`` tokens plus the first ``num_sink_tokens``
+    (not in the reference); pages behind it can be given back between steps
+    with ``pages.evict_window_pages``."""
     PagedAttnState.kv_pool = kv_pool
     PagedAttnState.page_size = page_size
     PagedAttnState.dtype = kv_pool.dtype
+    PagedAttnState.window_left = window_left
+    PagedAttnState.num_sink_tokens = num_sink_tokens
     PagedAttnState.workspace_buffer = torch.empty(WORKSPACE_BYTES, dtype=torch.uint8,
                                                   device=device)
-    PagedAttnState.prefill_wrapper = flashinfer.BatchPrefillWithPagedKVCacheWrapper(
-        PagedAttnState.workspace_buffer, "HND")
-    PagedAttnState.decode_wrapper = flashinfer.BatchDecodeWithPagedKVCacheWrapper(
-        PagedAttnState.workspace_buffer, "HND")
+    ws = PagedAttnState.workspace_buffer
+    if window_left is None:
+        if num_sink_tokens:
+            raise ValueError("num_sink_tokens needs a window_left")
+        PagedAttnState.prefill_wrapper = flashinfer.BatchPrefillWithPagedKVCacheWrapper(ws, "HND")
+        PagedAttnState.decode_wrapper = flashinfer.BatchDecodeWithPagedKVCacheWrapper(ws, "HND")
+        return
+    window = {"window_left": window_left, "num_sink_tokens": num_sink_tokens}
+    PagedAttnState.prefill_wrapper = flashinfer.BatchPrefillWithSlidingWindowWrapper(
+        ws, "HND", **window)
+    PagedAttnState.decode_wrapper = flashinfer.BatchDecodeWithSlidingWindowWrapper(
+        ws, "HND", **window)
 
 
 init_paged_attn_state = init_flashinfer_state
