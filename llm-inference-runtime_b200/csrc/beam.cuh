@@ -12,16 +12,18 @@
 // large traffic: bound by HBM), and a second launch joins the chunks of a
 // request.
 //
-// Chunk pass: a CTA holds a chunk in registers (all its loads in flight at
-// once) and takes the chunk's maximum and sum from them. Of its 256 threads'
-// maxima each warp's four best are looked at; the K-th of those 32 is a
-// threshold that at least K logits reach and few others do. The threads whose
-// maximum reaches it (about K of 256) have their logits read again, a word per
-// lane, and what passes is ranked by counting. Many more reach it only when
-// many are equal to it (masked or constant rows): then the ones above it and,
-// in index order, as many equal ones as are missing are taken. If more than
-// kBeamCap lie above it (a layout against the threads' order), K rounds of a
-// block-wide maximum give the same result.
+// Chunk pass: a CTA streams its chunk once, two 16-byte vectors a thread at a
+// time with six more on their way; each thread keeps its own maximum and
+// the sum relative to it, so nothing waits on another thread until the end.
+// Of the 256 threads' maxima each warp's four best are looked at; the K-th of
+// those 32 is a threshold that at least K logits reach and few others do. The
+// threads whose maximum reaches it (about K of 256) have the step that holds it
+// read again, a word per lane (all their logits if another step reaches it
+// too), and what passes is ranked by counting. Many threads
+// reach it only when many logits are equal to it (masked or constant rows):
+// then the ones above it and, in index order, as many equal ones as are missing
+// are taken. If more than kBeamCap lie above it (a layout against the threads'
+// order), K rounds of a block-wide maximum give the same result.
 #pragma once
 
 #include "pa_common.cuh"
@@ -35,13 +37,20 @@ constexpr int kBeamMaxBeams = 256;      // JoinKey's 8 bits
 constexpr int kBeamMaxVocab = 1 << 24;  // and 24
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kBeamCap = 1024;  // elements ranked by counting
+constexpr int kBeamMany = 128;  // threads at the threshold: many logits are equal to it
+constexpr int kBeamStep = 2;    // vectors of a thread taken together
+constexpr int kBeamRing = 4;    // such steps in flight
+constexpr float kBeamSlack = 5.f;
+constexpr int kBeamRingBytes = kBeamRing * kBeamStep * kBeamThreads * 16;
+static_assert(kBeamRingBytes >= kBeamCap * 8, "the ring holds the candidates at the end");
 
 struct BeamParams {
   const void* logits;
   int64_t stride_b, stride_w;  // elements
   const float* scores;         // [batch, beams]
   int64_t score_stride;
-  int32_t batch, beams, vocab, k, chunks;
+  int32_t batch, beams, vocab, k;
+  int32_t chunks, chunk_vectors;  // per row; 16-byte vectors of each thread per chunk
   double* part_off;   // [rows, chunks]: off, about max * log2(e); -inf: nothing finite
   double* part_sum;   // [rows, chunks]: sum of 2^(x log2(e) - off)
   uint64_t* part_key;  // [rows, chunks, k]: best first, 0: none
@@ -211,34 +220,37 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p, int bytes) {
   return v;
 }
 
-// One chunk of one row. Vector i of thread t holds logits chunk * CH +
-// (i * 256 + t) * N and the N - 1 after it whatever the row's alignment, so
-// equal rows give equal sums; places past the row hold -inf.
+// One chunk of one row. Vector i of thread t holds logits base + (i * 256 + t)
+// * N and the N - 1 after it whatever the row's alignment, so equal rows give
+// equal sums; places past the row hold -inf.
 //
-// Per logit: half an instruction of packed maxima and four for the sum (unpack,
-// fma, ex2, add). ex2 is the narrowest pipe (16 per SM and cycle). NaN needs no instruction of its
-// own: maxima and comparisons pass over it, and a thread whose sum comes out
-// NaN cleans its logits and adds them up again.
-template <typename T, int VPT>
+// Per logit: half an instruction of packed maxima and four for the sum
+// (unpack, fma, ex2, add). ex2 is the narrowest pipe (16 per
+// SM and cycle: 128256 logits of 512 rows take 14.4 us of it, and 20.1 us of
+// HBM). NaN needs no instruction of its own: maxima and comparisons pass over
+// it, and a thread whose sum is not finite adds its logits up again, cleaned.
+template <typename T>
 __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamParams p) {
   using W = BeamWord<T>;
   constexpr int N = 16 / sizeof(T);
-  constexpr int CH = kBeamThreads * N * VPT;
+  constexpr int kRow = kBeamThreads * N;  // logits per vector of all threads
   __shared__ alignas(16) uint32_t s_four[32];
   __shared__ uint64_t s_key[kBeamWarps];
-  __shared__ float s_sum[kBeamWarps];
+  __shared__ double s_sum[kBeamWarps];
   __shared__ int s_warp[kBeamWarps];
-  __shared__ uint64_t s_cand[kBeamCap];
-  __shared__ uint8_t s_who[kBeamThreads];
-  __shared__ int s_n, s_nwho;
+  extern __shared__ uint4 ring[];  // kBeamRing steps
+  uint64_t* const s_cand = reinterpret_cast<uint64_t*>(ring);  // [kBeamCap], once they are taken
+  __shared__ int s_who[kBeamThreads];
+  __shared__ int s_n, s_one, s_all;
   griddep_wait();
   griddep_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int chunk = blockIdx.x, w = blockIdx.y, b = blockIdx.z;
   const int64_t part = (static_cast<int64_t>(b) * p.beams + w) * p.chunks + chunk;
   const T* x = static_cast<const T*>(p.logits) + b * p.stride_b + w * p.stride_w;
-  const int base = chunk * CH, K = p.k;
-  if (tid == 0) s_n = s_nwho = 0;
+  const int base = chunk * p.chunk_vectors * kRow, K = p.k;
+  const int vectors = min(p.chunk_vectors, (p.vocab - base + kRow - 1) / kRow);  // > 0
+  if (tid == 0) s_n = s_one = s_all = 0;
   // a beam without a score continues nothing: all its logits count as -inf
   const float c0 = __ldg(p.scores + b * p.score_stride + w);
   const bool dead = !(c0 > -INFINITY);
@@ -259,66 +271,116 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
     }
     return r;
   };
-  uint32_t v[VPT][4];
-  const bool whole = !dead && base + CH <= p.vocab &&
-                     (reinterpret_cast<uintptr_t>(x + base) & 15) == 0;
+  // vectors whose logits of every thread are inside the row and aligned
+  const bool aligned = (reinterpret_cast<uintptr_t>(x + base) & 15) == 0;
+  const int whole = aligned && !dead ? min(vectors, (p.vocab - base) / kRow) : 0;
   const uint4* src = reinterpret_cast<const uint4*>(x + base) + tid;
+  float best = -INFINITY;
+  // the sum of 2^(x log2(e) - my_off), my_off = ref log2(e) rounded; ref
+  // follows the maximum only when it has grown by kBeamSlack (each time costs
+  // the sum one rounding of ex2)
+  float ref = -INFINITY, my_off = 0.f;
+  double my_sum = 0.0;
+  int best_step = 0;       // where `best` is
+  float second = -INFINITY;  // the largest logit of the other steps
+  auto take = [&](const uint4 (&in)[kBeamStep], int step) {
+    uint32_t v[kBeamStep][4];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const uint4 r = whole ? __ldcs(src + i * kBeamThreads) : load(i);
-    v[i][0] = r.x;
-    v[i][1] = r.y;
-    v[i][2] = r.z;
-    v[i][3] = r.w;
+    for (int u = 0; u < kBeamStep; ++u) {
+      v[u][0] = in[u].x;
+      v[u][1] = in[u].y;
+      v[u][2] = in[u].z;
+      v[u][3] = in[u].w;
+    }
+    uint32_t m2 = W::kNone;
+#pragma unroll
+    for (int u = 0; u < kBeamStep; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m2 = W::max2(m2, v[u][q]);
+    const float m = W::N == 2 ? fmaxf(W::at(m2, 0), W::at(m2, 1)) : W::at(m2, 0);
+    if (m > best) {
+      second = best;
+      best = m;
+      best_step = step;
+      if (m > ref + kBeamSlack) {
+        const float off = m * kLog2e;
+        my_sum *= ex2(my_off - off);  // (0 before the first finite logit)
+        ref = m;
+        my_off = off;
+      }
+    } else {
+      second = fmaxf(second, m);
+    }
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < kBeamStep; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < W::N; ++e)
+          part[(q * W::N + e) & 3] += ex2(fmaf(W::at(v[u][q], e), kLog2e, -my_off));
+    my_sum += (part[0] + part[1]) + (part[2] + part[3]);
+  };
+  // Steps of whole vectors first, through a ring of shared memory in which
+  // every thread copies and reads its own slots (no barrier), kBeamRing steps
+  // in flight. (Loads into registers, each behind its own bounds check, took
+  // 47 us where this takes 38: 512 rows of 128256 bf16.)
+  const int steps = whole / kBeamStep;
+  auto copy = [&](int step) {
+    if (step < steps) {
+#pragma unroll
+      for (int u = 0; u < kBeamStep; ++u)
+        copy_async16(ring + ((step % kBeamRing) * kBeamStep + u) * kBeamThreads + tid,
+                     src + (step * kBeamStep + u) * kBeamThreads);
+    }
+    copy_async_commit();  // (an empty group keeps the count)
+  };
+  uint4 now[kBeamStep];
+  for (int i = 0; i < kBeamRing; ++i) copy(i);
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    copy_async_wait<kBeamRing - 1>();
+#pragma unroll
+    for (int u = 0; u < kBeamStep; ++u)
+      now[u] = ring[((i % kBeamRing) * kBeamStep + u) * kBeamThreads + tid];
+    take(now, i);
+    copy(i + kBeamRing);
   }
-  auto clean_all = [&]() {
+  copy_async_wait<0>();
+#pragma unroll 1
+  for (int i = steps * kBeamStep; i < vectors; i += kBeamStep) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[i][q] = W::clean(v[i][q]);
-  };
-  auto thread_max = [&]() {
-    uint32_t m = W::kNone;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) m = W::max2(m, v[i][q]);
-    return W::N == 2 ? fmaxf(W::at(m, 0), W::at(m, 1)) : W::at(m, 0);
-  };
-  float best = thread_max();
-  if (best == INFINITY) {
-    clean_all();
-    best = thread_max();
+    for (int u = 0; u < kBeamStep; ++u)
+      now[u] = i + u < vectors ? load(i + u)
+                               : make_uint4(W::kNone, W::kNone, W::kNone, W::kNone);
+    take(now, i / kBeamStep);
   }
   // 0: no logit here. (+ 0.f: -0 and +0 are one value)
-  const uint32_t mine = base + tid * N < p.vocab ? order_bits(best + 0.f) : 0u;
+  const uint32_t mine =
+      base + tid * N < p.vocab ? order_bits(fminf(best, W::kMost) + 0.f) : 0u;
   uint32_t top;
   const uint32_t least = block_threshold(mine, K, s_four, lane, wid, &top);
   const float m = order_value(top);  // the chunk is not empty
-  // (s_nwho was set before the barrier above)
-  if (mine >= least && mine != 0) s_who[atomicAdd(&s_nwho, 1)] = static_cast<uint8_t>(tid);
+  // Threads at the threshold: usually with one step's logits only, which are
+  // listed from the front, otherwise from the back. (Both counters were set
+  // before the barrier above.)
+  if (mine >= least && mine != 0) {
+    const bool one = order_bits(fminf(second, W::kMost) + 0.f) < least;
+    const int at = one ? atomicAdd(&s_one, 1) : kBeamThreads - 1 - atomicAdd(&s_all, 1);
+    s_who[at] = best_step << 8 | tid;
+  }
 
   // this chunk's sum of 2^(x log2(e) - off), off = m log2(e) rounded: the join
   // takes the same off, so its rounding cancels
   const float off = m * kLog2e;
   const bool huge = fabsf(m) > 1e30f;  // the product may overflow; x - m does as well there
-  float sum = 0.f;
-  if (m != -INFINITY && !huge) {
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int e = 0; e < W::N; ++e)
-          part[(q * W::N + e) & 3] += ex2(fmaf(W::at(v[i][q], e), kLog2e, -off));
-    sum = (part[0] + part[1]) + (part[2] + part[3]);
-  }
-  if (m != -INFINITY && (huge || sum != sum)) {
-    // rare: from memory again, with NaN as -inf
-    sum = 0.f;
+  if (m == -INFINITY || best == -INFINITY) {
+    my_sum = 0.0;
+  } else if (huge || !(my_sum < 1e30)) {
+    // rare (NaN, infinite or huge logits): from memory again, cleaned
+    my_sum = 0.0;
 #pragma unroll 1
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < vectors; ++i) {
       const uint4 r = load(i);
       const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
 #pragma unroll
@@ -326,43 +388,53 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
 #pragma unroll
         for (int e = 0; e < W::N; ++e) {
           const float f = W::at(word[q], e);
-          sum += ex2(huge ? (f - m) * kLog2e : fmaf(f, kLog2e, -off));
+          my_sum += ex2(huge ? (f - m) * kLog2e : fmaf(f, kLog2e, -off));
         }
     }
+  } else {
+    my_sum *= ex2(my_off - off);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_sum[wid] = sum;
+  for (int o = 16; o > 0; o >>= 1) my_sum += __shfl_xor_sync(0xffffffffu, my_sum, o);
+  if (lane == 0) s_sum[wid] = my_sum;
   __syncthreads();
 
-  // the logits that reach the threshold, in any order: lane l reads word l of
-  // a thread's VPT * 4
+  // the logits that reach the threshold, in any order: the lanes read a
+  // thread's words
   auto index = [&](int i, int q, int e) {
     return base + (i * kBeamThreads + tid) * N + q * W::N + e;
   };
-  const int nwho = s_nwho;
-  if (!dead) {
-    for (int k = wid; k < nwho; k += kBeamWarps) {
+  const int ones = s_one, alls = s_all;
+  const bool many = ones + alls > kBeamMany || least <= order_bits(-INFINITY);
+  // word `word` of a thread's vectors
+  auto look = [&](int thread, int word) {
+    const int i = word >> 2, at = base + (i * kBeamThreads + thread) * N + (word & 3) * W::N;
+    if (i < whole) {  // both of a word at once; mostly neither passes
+      const uint32_t v2 = W::clean(__ldg(reinterpret_cast<const uint32_t*>(x + at)));
+      const float f = W::N == 2 ? fmaxf(W::at(v2, 0), W::at(v2, 1)) : W::at(v2, 0);
+      if (order_bits(f + 0.f) < least) return;
+    }
 #pragma unroll
-      for (int word = lane; word < VPT * 4; word += 32) {
-        const int at = base + ((word >> 2) * kBeamThreads + s_who[k]) * N + (word & 3) * W::N;
-        if (whole) {  // aligned: both of a word at once; mostly neither passes
-          const uint32_t v2 = W::clean(__ldg(reinterpret_cast<const uint32_t*>(x + at)));
-          const float f = W::N == 2 ? fmaxf(W::at(v2, 0), W::at(v2, 1)) : W::at(v2, 0);
-          if (order_bits(f + 0.f) < least) continue;
-        }
-#pragma unroll
-        for (int e = 0; e < W::N; ++e) {
-          if (at + e >= p.vocab) continue;
-          const float raw = static_cast<float>(__ldg(x + at + e));
-          const float f = fminf(raw, W::kMost) + 0.f;
-          if (raw == raw && order_bits(f) >= least) {
-            const int n = atomicAdd(&s_n, 1);
-            if (n < kBeamCap) s_cand[n] = beam_key(f, at + e);
-          }
-        }
+    for (int e = 0; e < W::N; ++e) {
+      if (at + e >= p.vocab) continue;
+      const float raw = static_cast<float>(__ldg(x + at + e));
+      const float f = fminf(raw, W::kMost) + 0.f;
+      if (raw == raw && order_bits(f) >= least) {
+        const int n = atomicAdd(&s_n, 1);
+        if (n < kBeamCap) s_cand[n] = beam_key(f, at + e);
       }
     }
+  };
+  if (!many) {
+    constexpr int kWords = kBeamStep * 4;  // a step's
+    for (int k = tid / kWords; k < ones; k += kBeamThreads / kWords) {
+      const int who = s_who[k], word = (who >> 8) * kWords + tid % kWords;
+      if (word < vectors * 4) look(who & 255, word);
+    }
+    for (int k = wid; k < alls; k += kBeamWarps)
+#pragma unroll 2
+      for (int word = lane; word < vectors * 4; word += 32)
+        look(s_who[kBeamThreads - 1 - k] & 255, word);
   }
   __syncthreads();
   if (tid == 0) {
@@ -374,7 +446,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
   }
   uint64_t* out = p.part_key + part * K;
   int n = s_n;
-  if (n > kBeamCap || least <= order_bits(-INFINITY)) {
+  if (many || n > kBeamCap) {
     // many equal the threshold (or NaN counts as -inf, which nothing above
     // has seen): from memory again, first those above it
     __syncthreads();
@@ -382,7 +454,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
     __syncthreads();
     const uint32_t equal = max(least, order_bits(-INFINITY));
 #pragma unroll 1
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < vectors; ++i) {
       const uint4 r = load(i);
       const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
 #pragma unroll
@@ -400,7 +472,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
     n = s_n;
     // then the first equal ones: vector i of all threads comes before i + 1
 #pragma unroll 1
-    for (int i = 0; i < VPT && n < K; ++i) {  // n: the same for every thread
+    for (int i = 0; i < vectors && n < K; ++i) {  // n: the same for every thread
       const uint4 r = load(i);
       const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
       uint32_t mask = 0;  // which of the vector's logits are equal
@@ -444,9 +516,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
   uint64_t last = ~0ULL;
 #pragma unroll 1
   for (int k = 0; k < K; ++k) {
-    uint64_t next = 0;
+    uint64_t best_key = 0;
 #pragma unroll 1
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < vectors; ++i) {
       const uint4 r = load(i);
       const uint32_t word[4] = {W::clean(r.x), W::clean(r.y), W::clean(r.z), W::clean(r.w)};
 #pragma unroll
@@ -454,10 +526,10 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
 #pragma unroll
         for (int e = 0; e < W::N; ++e) {
           const uint64_t key = beam_key(W::at(word[q], e) + 0.f, index(i, q, e));
-          if (index(i, q, e) < p.vocab && key < last && key > next) next = key;
+          if (index(i, q, e) < p.vocab && key < last && key > best_key) best_key = key;
         }
     }
-    last = block_max<uint64_t>(next, s_key, lane, wid);
+    last = block_max<uint64_t>(best_key, s_key, lane, wid);
     if (tid == 0) out[k] = last;
   }
 }

@@ -771,27 +771,26 @@ int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
 
 namespace {
 
-// Vectors per thread of the chunk pass. Every chunk costs about as much beside
-// its loads as 32 logits a thread do, and a list for the join, so chunks are
-// large (8 vectors: 64 requests x 8 beams x 128256 bf16 logits take 47 us, 65
-// with 4 vectors, 102 with 2; 8 beams of one request 9.8, 12.3 and 18.7). Only
-// when chunks of 2 vectors fill no more than the SMs once are they no slower:
-// 4 beams of 32000 then take 7.0 us and 7.6 with 8 vectors.
-template <typename T>
-int beam_vectors(int64_t rows, int vocab, int sms) {
-  const int ch = kBeamThreads * static_cast<int>(16 / sizeof(T)) * 2;
-  return rows * ((vocab + ch - 1) / ch) <= sms ? 2 : 8;
-}
+// How a row is cut: chunks per row, and 16-byte vectors of each thread per
+// chunk. Enough chunks for four CTAs per SM, unless that makes the join's
+// candidates (beams x chunks x k) more than its threads hold: 8 beams of one
+// request over 128256 bf16 logits take 18.1 us in 32 chunks a row, 12.5 in 16
+// and 10.2 in 8; 64 such requests 38.2 us with this target, 45.5 with one CTA
+// per SM and 44.4 with sixteen.
+struct BeamCut {
+  int chunks, vectors;
+};
 
-template <typename T>
-int beam_chunk_elements(int64_t rows, int vocab, int sms) {
-  return kBeamThreads * static_cast<int>(16 / sizeof(T)) * beam_vectors<T>(rows, vocab, sms);
-}
-
-int beam_chunks(int dtype, int64_t rows, int vocab, int sms) {
-  const int ch = dtype == PA_DTYPE_F32 ? beam_chunk_elements<float>(rows, vocab, sms)
-                                       : beam_chunk_elements<__half>(rows, vocab, sms);
-  return (vocab + ch - 1) / ch;
+BeamCut beam_cut(int dtype, int batch, int beams, int vocab, int k, int sms) {
+  const int row = kBeamThreads * (dtype == PA_DTYPE_F32 ? 4 : 8);  // logits per vector of all
+  const int all = (vocab + row - 1) / row;
+  const int64_t rows = std::max<int64_t>(1, static_cast<int64_t>(batch) * beams);
+  const int64_t most = std::max<int64_t>(4, kBeamThreads * kBeamHeld / (beams * k));
+  const int64_t want = std::max<int64_t>(1, std::min((4 * sms + rows - 1) / rows, most));
+  BeamCut c;
+  c.vectors = static_cast<int>(std::max<int64_t>((all + want - 1) / want, kBeamStep));
+  c.chunks = (all + c.vectors - 1) / c.vectors;
+  return c;
 }
 
 struct BeamWsLayout {
@@ -806,13 +805,6 @@ BeamWsLayout beam_ws_layout(int64_t rows, int chunks, int k) {
   L.key = 2 * L.off;
   L.total = L.key + align256(n * k * sizeof(uint64_t));
   return L;
-}
-
-template <typename T>
-int launch_beam(const BeamParams& p, int vectors, cudaStream_t s) {
-  const dim3 grid(p.chunks, p.beams, p.batch), block(kBeamThreads);
-  return vectors == 2 ? launch_chain(beam_chunk_kernel<T, 2>, grid, block, 0, s, p)
-                      : launch_chain(beam_chunk_kernel<T, 8>, grid, block, 0, s, p);
 }
 
 int check_beam(int batch, int beams, int vocab, int k, int dtype) {
@@ -834,7 +826,10 @@ size_t pa_beam_select_workspace_bytes(int32_t batch_size, int32_t num_beams, int
   const int dev = current_device();
   const int sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
   const int64_t rows = static_cast<int64_t>(batch_size) * num_beams;
-  return beam_ws_layout(rows, beam_chunks(dtype, rows, vocab_size, sms), num_candidates).total;
+  return beam_ws_layout(
+             rows, beam_cut(dtype, batch_size, num_beams, vocab_size, num_candidates, sms).chunks,
+             num_candidates)
+      .total;
 }
 
 int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_stride_w,
@@ -852,9 +847,9 @@ int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_s
   const int dev = current_device();
   const int sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
   const int64_t rows = static_cast<int64_t>(batch_size) * num_beams;
-  const int chunks = beam_chunks(dtype, rows, vocab_size, sms);
+  const BeamCut cut = beam_cut(dtype, batch_size, num_beams, vocab_size, num_candidates, sms);
   if (batch_size > 65535) return PA_ERR_UNSUPPORTED;  // the grid's third dimension
-  const BeamWsLayout L = beam_ws_layout(rows, chunks, num_candidates);
+  const BeamWsLayout L = beam_ws_layout(rows, cut.chunks, num_candidates);
   if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   BeamParams p;
@@ -867,7 +862,8 @@ int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_s
   p.beams = num_beams;
   p.vocab = vocab_size;
   p.k = num_candidates;
-  p.chunks = chunks;
+  p.chunks = cut.chunks;
+  p.chunk_vectors = cut.vectors;
   p.part_off = reinterpret_cast<double*>(ws + L.off);
   p.part_sum = reinterpret_cast<double*>(ws + L.sum);
   p.part_key = reinterpret_cast<uint64_t*>(ws + L.key);
@@ -875,13 +871,15 @@ int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_s
   p.out_parents = out_parents;
   p.out_tokens = out_tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc;
-  if (dtype == PA_DTYPE_F32)
-    rc = launch_beam<float>(p, beam_vectors<float>(rows, vocab_size, sms), s);
-  else if (dtype == PA_DTYPE_BF16)
-    rc = launch_beam<__nv_bfloat16>(p, beam_vectors<__nv_bfloat16>(rows, vocab_size, sms), s);
-  else
-    rc = launch_beam<__half>(p, beam_vectors<__half>(rows, vocab_size, sms), s);
+  const dim3 grid(cut.chunks, num_beams, batch_size), block(kBeamThreads);
+  static std::atomic<uint64_t> done[3];
+  auto go = [&](auto kernel, std::atomic<uint64_t>* mask) -> int {
+    if (allow_smem(kernel, kBeamRingBytes, mask, dev) != cudaSuccess) return PA_ERR_CUDA;
+    return launch_chain(kernel, grid, block, kBeamRingBytes, s, p);
+  };
+  const int rc = dtype == PA_DTYPE_F32    ? go(beam_chunk_kernel<float>, &done[0])
+                 : dtype == PA_DTYPE_BF16 ? go(beam_chunk_kernel<__nv_bfloat16>, &done[1])
+                                          : go(beam_chunk_kernel<__half>, &done[2]);
   if (rc != PA_OK) return rc;
   const size_t smem = static_cast<size_t>(num_beams) * 16;
   return launch_chain(beam_join_kernel, dim3(batch_size), dim3(kBeamThreads), smem, s, p);

@@ -231,6 +231,20 @@ template <int N>
 __device__ __forceinline__ void bulk_wait_read_but() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
+// One thread's 16-byte copies global -> shared (both aligned), counted in
+// groups; a group's bytes are visible to the thread that waited for it.
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src))
+               : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 // Untiled bulk copies: both addresses 16-byte aligned, bytes a multiple of 16.
 // The load completes on `bar`, the store belongs to the thread's bulk group.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,

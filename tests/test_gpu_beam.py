@@ -1,10 +1,14 @@
 """Beam selection against a plain 64-bit implementation, and a beam search
 over the paged cache against one that keeps every beam's keys.
 
-Choices are whole numbers and are equal. Scores: the sum of exponentials is
-off by at most 2^-21 relative (fp32 exponentials, each 2^-22), which is 5e-7 in
-its logarithm; that is rounded to fp32 (2^-24 |lse|), and so is the score
-(2^-24 |score|)."""
+Choices are whole numbers and are equal. Scores: a summand 2^(x log2(e) - off)
+carries the rounding of its exponent (below 8 for the summands that matter:
+2^-22 ln 2 relative), of log2(e) and of the exponential (2^-22 each), its
+thread's four fp32 additions (2^-24 each) and the exponential that joins the
+thread to the others (2^-22): together below 1.2e-6 of the sum, which is as much
+in its logarithm. That is rounded to fp32 (2^-24 |lse|), and so is the score
+(2^-24 |score|).
+"""
 
 from __future__ import annotations
 
@@ -44,7 +48,7 @@ def plain_select(logits, scores, n):
                 continue
             lse = np.float32(top + math.log(np.exp(x[b, w] - top).sum()))
             flat.append(c[b, w] + (x[b, w] - np.float64(lse)))
-            near.append(5e-7 + 2.0 ** -24 * abs(float(lse)) * 2)
+            near.append(1.2e-6 + 2.0 ** -24 * abs(float(lse)) * 2)
         flat = np.concatenate(flat)
         # best score, lowest beam, largest logit, lowest token
         index = np.arange(beams * vocab)
