@@ -203,9 +203,10 @@ int pa_fork_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
  *   block_tables[rows][max_blocks], rows block_table_stride elements apart:
  *     page of tokens [j * page_size, (j + 1) * page_size) of a row, -1 = given back
  *   seq_lens[rows]          tokens a row holds; its entries j < ceil(len / page_size)
- * Counting errors that only the device sees (a page id outside the pool, a
- * count that would fall below zero, no free page left) are added to counts[2]
- * and recorded as PA_ERR_DEVICE_CHECK; sound rows are processed all the same.
+ * Errors that only the device sees (a page id outside the pool, a count that
+ * falls below zero, no free page left) are recorded as PA_ERR_DEVICE_CHECK and
+ * counted in counts[2] where its line says so; sound rows are processed all
+ * the same.
  *
  * pa_release_pages, window_left >= 0: entries of pages that lie wholly behind
  * the window of the row's last token, that is

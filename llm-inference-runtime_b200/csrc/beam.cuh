@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
       second = best;
       best = m;
       best_step = step;
-      if (m > ref + kBeamSlack) {
+      // (logits masked by the type's lowest value are no reference: their sum
+      // is 0 beside any other's)
+      if (m > ref + kBeamSlack && m > -1e30f) {
         const float off = m * kLog2e;
         my_sum *= ex2(my_off - off);  // (0 before the first finite logit)
         ref = m;

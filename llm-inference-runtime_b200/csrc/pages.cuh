@@ -342,12 +342,12 @@ __global__ void __launch_bounds__(kForkThreads) fork_rows_kernel(const ForkSeqPa
       for (int j = tid; j < full; j += kForkThreads) {
         const int page = __ldg(row + j);
         if (page < 0) continue;
-        if (page < p.num_pages)
-          atomicAdd(p.refs + page, delta);
-        else
+        // (sound counts stay >= 0 in any order: each holder leaves only once)
+        if (page >= p.num_pages || atomicAdd(p.refs + page, delta) + delta < 0)
           set_status(PA_ERR_DEVICE_CHECK);
       }
-    if (tid == 0 && len % p.page_size && usable && last >= 0) atomicSub(p.refs + last, 1);
+    if (tid == 0 && len % p.page_size && usable && last >= 0 && atomicSub(p.refs + last, 1) <= 0)
+      set_status(PA_ERR_DEVICE_CHECK);
   }
   // row r as a child: the parent's full pages
   const ForkRow f = fork_row(p, r);

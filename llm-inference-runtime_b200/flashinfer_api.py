@@ -57,12 +57,14 @@ def _as_dtype(dt) -> Optional[torch.dtype]:
 
 # The stream handle and the current device's number without the objects that
 # torch.cuda.current_stream() builds (3 us of a 10 us call).
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _SAME_DEVICE = contextlib.nullcontext()
 
 
 def _stream() -> int:
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
     return _raw_stream(_current_device())
 
 

@@ -315,6 +315,51 @@ def test_fork_reports_unsound_rows(pages, fi, lir):
     assert c.tolist() == [1, 1, 0, 1, 1, 1, 0, 0]
 
 
+@pytest.mark.parametrize("length", [32, 20])
+def test_fork_reports_counts_below_zero(pages, length):
+    """A row that nobody continues gives up pages that no count holds."""
+    tables, lens = _i32([[0, 1, -1], [2, 3, -1]]), _i32([length, length])
+    refs = _i32([1, 1, 0, 0, 0, 0])
+    with pytest.raises(RuntimeError, match="device"):
+        pages.fork_sequences(_pool(6), tables, lens, _i32([0, 0]), refs)
+
+
+def test_evict_and_compact_captured_and_replayed(pages, fi, lir):
+    tables, lens, refs, _ = _random_state(95, 20, 600, spare=50, external=0.0, gone=0.0)
+    pool = _pool(len(refs), 2)
+    fresh, t, n, c = pool.clone(), _i32(tables), _i32(lens), _i32(refs)
+    fi._CHECK, saved = False, fi._CHECK
+    try:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            pages.evict_window_pages(t, n, c, 2 ** 31 - 1)
+            pages.compact_pages(fresh.clone(), t.clone(), n, c.clone())
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            evicted = pages.evict_window_pages(t, n, c, 100, 4)
+            remap, counts = pages.compact_pages(pool, t, n, c)
+        for seed in (1, 2):
+            lens = np.maximum(lens - seed, 0)
+            n.copy_(_i32(lens))
+            t.copy_(_i32(tables))
+            c.copy_(_i32(refs))
+            pool.copy_(fresh)
+            graph.replay()
+            torch.cuda.synchronize()
+            want_t, want_r, want_e = plain_release(tables, lens, refs, 100, 4)
+            want_t, want_r, want_m, want_c, copies = plain_compact(want_t, lens, want_r)
+            assert evicted.tolist() == want_e and counts.tolist() == want_c
+            assert np.array_equal(t.cpu().numpy(), want_t)
+            assert np.array_equal(c.cpu().numpy(), want_r)
+            assert np.array_equal(remap.cpu().numpy(), want_m)
+            assert torch.equal(_bits(pool), _bits(_copied(fresh, copies)))
+        assert lir._lib.device_status() == 0
+    finally:
+        fi._CHECK = saved
+
+
 def test_fork_captured_and_replayed(pages, fi, lir):
     tables, lens, refs, rng = _random_state(91, 30, 300, spare=60)
     pool = _pool(len(refs), 2)
