@@ -580,6 +580,29 @@ def _check_window(window_left, num_sink_tokens) -> Tuple[int, int]:
     return window_left, num_sink_tokens
 
 
+def _check_run_tensors(wrapper, q: torch.Tensor, paged_kv_cache, out, lse, append) -> None:
+    """What the kernels cannot see: tensors of another device than the
+    workspace, outputs of another type."""
+    if not wrapper._planned:
+        raise RuntimeError("plan() must be called before run()")
+    gpu = wrapper._ws.get_device()  # -1 for what is not on a GPU
+    fits = q.get_device() == gpu
+    if isinstance(paged_kv_cache, torch.Tensor):
+        fits = fits and paged_kv_cache.get_device() == gpu
+    else:
+        fits = fits and all(t.get_device() == gpu for t in paged_kv_cache)
+    if append is not None:
+        fits = fits and append[0].get_device() == gpu and append[1].get_device() == gpu
+    if not fits:
+        raise ValueError(f"every tensor must be on the workspace's device, {wrapper._ws.device}")
+    if out is not None and (out.dtype != q.dtype or out.get_device() != gpu):
+        raise ValueError("out must have q's dtype and device")
+    if lse is not None and not (lse.dtype == torch.float32 and lse.get_device() == gpu
+                                and lse.dim() == 2 and lse.size(0) == q.size(0)
+                                and lse.size(1) == q.size(1) and lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 [rows, num_qo_heads] tensor")
+
+
 class BatchDecodeWithSlidingWindowWrapper(BatchDecodeWithPagedKVCacheWrapper):
     """Batched decode in which request b's query, at position ``kv_len - 1``,
     sees key j iff ``kv_len - 1 - j <= window_left`` or ``j < num_sink_tokens``
@@ -598,22 +621,28 @@ class BatchDecodeWithSlidingWindowWrapper(BatchDecodeWithPagedKVCacheWrapper):
         self._window, self._sinks = _check_window(window_left, num_sink_tokens)
 
     def _plan_call(self) -> int:
-        return _lib.load().pa_window_decode_plan(
-            _p(self._indptr), _p(self._indices), _p(self._last), self._batch,
-            self._indices.numel(), self._hq, self._hkv, self._d, self._p, self._window,
-            self._sinks, _p(self._ws), self._ws.numel() * self._ws.element_size(), _stream())
+        with _device_guard(self._ws.device):
+            return _lib.load().pa_window_decode_plan(
+                _p(self._indptr), _p(self._indices), _p(self._last), self._batch,
+                self._indices.numel(), self._hq, self._hkv, self._d, self._p, self._window,
+                self._sinks, _p(self._ws), self._ws.numel() * self._ws.element_size(), _stream())
+
+    def _run(self, q, paged_kv_cache, append, q_scale, k_scale, v_scale, out, lse, return_lse):
+        _check_run_tensors(self, q, paged_kv_cache, out, lse, append)
+        return super()._run(q, paged_kv_cache, append, q_scale, k_scale, v_scale, out, lse,
+                            return_lse)
 
     def _run_call(self, q, qsn, qsh, desc, append, scale, out, lse) -> int:
         table = (ctypes.byref(desc), _p(self._indices), _p(self._indptr), _p(self._last),
                  self._batch, self._indices.numel(), self._hq, self._window, self._sinks, scale,
-                 _p(self._ws), self._ws.numel() * self._ws.element_size(), _p(out), _p(lse),
-                 _stream())
-        if append is None:
-            return _lib.load().pa_window_decode_run(_p(q), qsn, qsh, *table)
-        k, v, pos = append
-        return _lib.load().pa_window_decode_append_run(
-            _p(q), qsn, qsh, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
-            _p(pos), *table)
+                 _p(self._ws), self._ws.numel() * self._ws.element_size(), _p(out), _p(lse))
+        with _device_guard(self._ws.device):
+            if append is None:
+                return _lib.load().pa_window_decode_run(_p(q), qsn, qsh, *table, _stream())
+            k, v, pos = append
+            return _lib.load().pa_window_decode_append_run(
+                _p(q), qsn, qsh, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
+                _p(pos), *table, _stream())
 
 
 class BatchPrefillWithSlidingWindowWrapper(BatchPrefillWithPagedKVCacheWrapper):
@@ -630,17 +659,24 @@ class BatchPrefillWithSlidingWindowWrapper(BatchPrefillWithPagedKVCacheWrapper):
         self._window, self._sinks = _check_window(window_left, num_sink_tokens)
 
     def _plan_call(self, total_qo: int) -> int:
-        return _lib.load().pa_window_prefill_plan(
-            _p(self._qo_indptr), _p(self._indptr), _p(self._last), self._batch, total_qo,
-            self._indices.numel(), self._hq, self._hkv, self._d, self._p, self._window,
-            self._sinks, _p(self._ws), self._ws.numel() * self._ws.element_size(), _stream())
+        with _device_guard(self._ws.device):
+            return _lib.load().pa_window_prefill_plan(
+                _p(self._qo_indptr), _p(self._indptr), _p(self._last), self._batch, total_qo,
+                self._indices.numel(), self._hq, self._hkv, self._d, self._p, self._window,
+                self._sinks, _p(self._ws), self._ws.numel() * self._ws.element_size(), _stream())
+
+    def run(self, q: torch.Tensor, paged_kv_cache, *args, out: Optional[torch.Tensor] = None,
+            lse: Optional[torch.Tensor] = None, **kwargs):
+        _check_run_tensors(self, q, paged_kv_cache, out, lse, None)
+        return super().run(q, paged_kv_cache, *args, out=out, lse=lse, **kwargs)
 
     def _run_call(self, q, qsn, qsh, desc, total_qo, scale, out, lse) -> int:
-        return _lib.load().pa_window_prefill_run(
-            _p(q), qsn, qsh, ctypes.byref(desc), _p(self._qo_indptr), _p(self._indices),
-            _p(self._indptr), _p(self._last), self._batch, total_qo, self._hq,
-            int(self._causal), self._window, self._sinks, scale, _p(self._ws),
-            self._ws.numel() * self._ws.element_size(), _p(out), _p(lse), _stream())
+        with _device_guard(self._ws.device):
+            return _lib.load().pa_window_prefill_run(
+                _p(q), qsn, qsh, ctypes.byref(desc), _p(self._qo_indptr), _p(self._indices),
+                _p(self._indptr), _p(self._last), self._batch, total_qo, self._hq,
+                int(self._causal), self._window, self._sinks, scale, _p(self._ws),
+                self._ws.numel() * self._ws.element_size(), _p(out), _p(lse), _stream())
 
 
 class MultiLevelCascadeAttentionWrapper:

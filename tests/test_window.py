@@ -80,3 +80,44 @@ def test_window_calls_check_their_arguments(lir):
         None) == E.PA_ERR_INVALID_ARGUMENT
     desc.head_dim = 96
     assert run() == E.PA_ERR_UNSUPPORTED
+
+
+class _OnGpu:
+    """A stand-in for a tensor of GPU 0, where there is none."""
+
+    device = "cuda:0"
+
+    def __init__(self, like):
+        self._like = like
+
+    def __getattr__(self, name):
+        return getattr(self._like, name)
+
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("name", ["BatchDecodeWithSlidingWindowWrapper",
+                                  "BatchPrefillWithSlidingWindowWrapper"])
+def test_run_refuses_tensors_that_do_not_fit(api, name):
+    """Other devices than the workspace's, outputs of another type or shape."""
+    w = getattr(api, name)(_OnGpu(torch.empty(16, dtype=torch.uint8)), "HND", window_left=4)
+    w._planned = True  # as after a plan
+    q = torch.zeros(2, 8, 64, dtype=torch.bfloat16)
+    pool = torch.zeros(4, 2, 2, 16, 64, dtype=torch.bfloat16)
+    halves = (pool[:, 0], pool[:, 1])
+    lse = torch.zeros(2, 8)
+    on = _OnGpu
+    for bad in ((q, pool), (on(q), pool), (on(q), halves), (on(q), (on(halves[0]), halves[1])),
+                (q, (on(halves[0]), on(halves[1])))):
+        with pytest.raises(ValueError, match="device"):
+            w.run(*bad)
+    cache = (on(halves[0]), on(halves[1]))
+    for out in (on(q.float()), q):
+        with pytest.raises(ValueError, match="out"):
+            w.run(on(q), cache, out=out)
+    for bad in (lse.double(), lse[:1], lse.t().contiguous().t(), lse[0]):
+        with pytest.raises(ValueError, match="lse"):
+            w.run(on(q), cache, lse=on(bad))
+    with pytest.raises(ValueError, match="lse"):
+        w.run(on(q), cache, lse=lse)
