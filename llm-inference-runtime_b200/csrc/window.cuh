@@ -122,6 +122,7 @@ struct FreshIndptr {
 };
 
 constexpr int kWindowPlanThreads = 1024;
+constexpr int kWindowRows = 64;
 
 // CTA 0 scans the requests' visible pages into the compacted indptr, records
 // each request's hole and cuts the stream into runs (decode_plan_block).
@@ -203,15 +204,25 @@ __global__ void __launch_bounds__(kWindowPlanThreads)
   int at = 0;
 #pragma unroll
   for (int w = 0; w < 32; ++w) at += s_warp[w];
-  for (int b = b0; b < b1; ++b) {
-    const WindowRow r =
-        window_row(kv_indptr, last_len, b, num_indices, page_size, window, sinks);
-    for (int v = tid; v < r.visible; v += kWindowPlanThreads) {
-      const int j = r.base + v + (v < r.span.sink_pages ? 0 : r.span.shift);
-      // a malformed table (which CTA 0 reports) may claim more than there is
-      if (at + v < L.capacity) out_indices[at + v] = __ldg(kv_indices + j);
+  // the range's rows, kWindowRows at a time, read by a thread each
+  __shared__ int4 s_row[kWindowRows];  // {first table entry, visible pages, sink pages, shift}
+  for (int g = b0; g < b1; g += kWindowRows) {
+    const int n = min(kWindowRows, b1 - g);
+    if (tid < n) {
+      const WindowRow r =
+          window_row(kv_indptr, last_len, g + tid, num_indices, page_size, window, sinks);
+      s_row[tid] = make_int4(r.base, r.visible, r.span.sink_pages, r.span.shift);
     }
-    at += r.visible;
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+      const int4 r = s_row[i];
+      for (int v = tid; v < r.y; v += kWindowPlanThreads)
+        // a malformed table (which CTA 0 reports) may claim more than there is
+        if (at + v < L.capacity)
+          out_indices[at + v] = __ldg(kv_indices + r.x + v + (v < r.z ? 0 : r.w));
+      at += r.y;
+    }
+    __syncthreads();  // s_row may be written again
   }
 }
 

@@ -481,3 +481,30 @@ def test_pages_on_another_stream(pages, fi, lir):
         assert lir._lib.device_status() == 0
     finally:
         fi._CHECK = saved
+
+
+def test_offsets_past_32_bits(pages):
+    """Pages whose bytes lie more than 4 GiB into the pool, and layers too."""
+    n, layers = 1300, 60  # 64 KB pages: 5.1 GB, 85 MB a layer
+    pool = torch.empty((layers, n, 2, 8, P, 128), dtype=torch.bfloat16, device=DEV)
+    bits = pool.view(torch.int16)
+    bits[:] = torch.arange(n, dtype=torch.int16, device=DEV)[None, :, None, None, None, None]
+    bits += (torch.arange(layers, device=DEV) * 500).to(torch.int16)[:, None, None, None, None, None]
+    refs = np.zeros(n, dtype=np.int64)
+    refs[[0, 5, n - 1, n - 2]] = [1, 2, 1, 1]
+    tables = np.array([[0, n - 1, -1], [5, n - 2, -1], [5, -1, -1]])
+    lens = np.array([20, 32, 16])
+    want_t, _, want_r, want_c, copies = plain_fork(tables, lens, refs, [0, 0, 1])
+    c = _i32(refs)
+    t, _, counts = pages.fork_sequences(pool, _i32(tables), _i32(lens), _i32([0, 0, 1]), c)
+    assert counts.tolist() == want_c and copies == [(n - 1, 1)]
+    assert np.array_equal(t.cpu().numpy(), want_t) and np.array_equal(c.cpu().numpy(), want_r)
+    layer = (torch.arange(layers, device=DEV) * 500).to(torch.int16)
+    same = lambda page, was: (bits[:, page].flatten(1) == (layer + was).to(torch.int16)[:, None]).all()  # noqa: E731
+    assert same(1, n - 1) and same(2, 2) and same(n - 1, n - 1)
+    lens = np.array([20, 20, 32])
+    want_t, want_r, want_m, want_c, copies = plain_compact(want_t, lens, want_r)
+    remap, counts = pages.compact_pages(pool, t, _i32(lens), c)
+    assert counts.tolist() == want_c and np.array_equal(remap.cpu().numpy(), want_m)
+    for s, d in copies:
+        assert same(d, s)

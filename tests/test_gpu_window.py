@@ -288,6 +288,35 @@ def test_two_runs_on_one_plan_are_bit_identical(fi):
     pr.check(a)
 
 
+def test_pages_past_32_bits_of_the_pool(fi):
+    """The visible pages are the last ones of a pool of more than 4 GiB."""
+    pr = _decode_problem([700, 90], 32, 8, 128, 200, 4, seed=43)
+    n = 70000  # 64 KB pages
+    pool = torch.full((n, 2, 8, P, 128), math.nan, dtype=torch.bfloat16, device=DEV)
+    held = pr.pool.shape[0]
+    pool[n - held:] = pr.pool.to(DEV)
+    pr.indices = np.where(pr.indices >= 0, pr.indices + n - held, -1)
+    q = pr.q.to(DEV)
+    w = _decode_wrapper(fi, pr)
+    pr.check(*w.run(q, pool, return_lse=True))
+    pos = _t([699, 89])
+    k = torch.randn((2, 8, 128), generator=torch.Generator().manual_seed(45)).to(pr.dtype).to(DEV)
+    out = w.run_with_append(q, pool, k, k, pos)
+    for b, at in enumerate((699, 89)):
+        page = int(pr.indices[int(pr.indptr[b]) + at // P])
+        assert page > 65536 and torch.equal(pool[page, 0, :, at % P], k[b])
+        pr.k64[b][:, at] = k[b].double().cpu()
+        pr.v64[b][:, at] = k[b].double().cpu()
+    pr.check(out)
+    pre = Problem([70, 3], [700, 90], 32, 8, 128, 200, 4, seed=44)
+    pool[:] = math.nan
+    held = pre.pool.shape[0]
+    pool[n - held:] = pre.pool.to(DEV)
+    pre.indices = np.where(pre.indices >= 0, pre.indices + n - held, -1)
+    pre.device_pool = lambda: pool
+    pre.check(*_prefill(fi, pre))
+
+
 # ---------------------------------------------------------------------- prefill
 def _prefill(fi, pr, return_lse=True):
     w = fi.BatchPrefillWithSlidingWindowWrapper(_ws(), pr.layout, window_left=pr.window,
