@@ -104,28 +104,28 @@ def kv_cache_desc(paged_kv_cache, kv_layout: str = "NHD") -> _lib.PagedKVCache:
     if isinstance(paged_kv_cache, torch.Tensor):
         if paged_kv_cache.dim() != 5 or paged_kv_cache.size(1) != 2:
             raise ValueError("paged_kv_cache tensor must be 5-D [num_pages, 2, ...]")
-        shape, stride = paged_kv_cache.shape, paged_kv_cache.stride()
-        shape, stride = shape[:1] + shape[2:], stride[:1] + stride[2:]
+        n, _, *shape = paged_kv_cache.shape
+        page_stride, kv_stride, *stride = paged_kv_cache.stride()
         dtype = paged_kv_cache.dtype
         k_ptr = paged_kv_cache.data_ptr()
-        v_ptr = k_ptr + paged_kv_cache.stride(1) * paged_kv_cache.element_size()
+        v_ptr = k_ptr + kv_stride * paged_kv_cache.element_size()
     else:
         k, v = paged_kv_cache
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError("k_cache / v_cache must be 4-D tensors of equal shape")
         if k.stride() != v.stride():
             raise ValueError("k_cache and v_cache must have the same strides")
-        shape, stride, dtype = k.shape, k.stride(), k.dtype
+        (n, *shape), (page_stride, *stride), dtype = k.shape, k.stride(), k.dtype
         k_ptr, v_ptr = k.data_ptr(), v.data_ptr()
-    if stride[3] != 1:
+    if stride[2] != 1:
         raise ValueError("the head_dim dimension of the KV cache must be contiguous")
     if kv_layout == "HND":
-        n, h, p, d = shape
-        head_stride, token_stride = stride[1], stride[2]
+        h, p, d = shape
+        head_stride, token_stride, _ = stride
     else:
-        n, p, h, d = shape
-        token_stride, head_stride = stride[1], stride[2]
-    return _lib.PagedKVCache(k_ptr, v_ptr, stride[0], head_stride, token_stride, n, h, p, d,
+        p, h, d = shape
+        token_stride, head_stride, _ = stride
+    return _lib.PagedKVCache(k_ptr, v_ptr, page_stride, head_stride, token_stride, n, h, p, d,
                              _dtype_code(dtype))
 
 
@@ -331,10 +331,16 @@ class BatchDecodeWithPagedKVCacheWrapper:
         self._q_dtype = _as_dtype(data_type) or _as_dtype(q_data_type)
         self._kv_dtype = _as_dtype(kv_data_type) or self._q_dtype
         self._sm_scale = sm_scale
-        what = type(self).__name__ + ".plan"
-        _lib.check(self._plan_call(), what)
-        _after(what)
+        rc = self._plan_call()
+        if rc or _CHECK:
+            self._report(rc, ".plan")
         self._planned = True
+
+    def _report(self, rc: int, call: str) -> None:
+        """Raises for a failing status, or with PA_CHECK for the device's."""
+        what = type(self).__name__ + call
+        _lib.check(rc, what)
+        _after(what)
 
     def _plan_call(self) -> int:
         return _lib.load().pa_decode_plan(
@@ -395,9 +401,9 @@ class BatchDecodeWithPagedKVCacheWrapper:
             lse = torch.empty((self._batch, self._hq), dtype=torch.float32, device=q.device)
         scale = self._sm_scale if self._sm_scale is not None else 1.0 / math.sqrt(self._d)
         scale *= _check_scales(q_scale, k_scale, v_scale)
-        what = type(self).__name__ + (".run" if append is None else ".run_with_append")
-        _lib.check(self._run_call(q, qsn, qsh, desc, append, float(scale), out, lse), what)
-        _after(what)
+        rc = self._run_call(q, qsn, qsh, desc, append, float(scale), out, lse)
+        if rc or _CHECK:
+            self._report(rc, ".run" if append is None else ".run_with_append")
         return (out, lse) if return_lse else out
 
     def _run_call(self, q, qsn, qsh, desc, append, scale, out, lse) -> int:
@@ -500,9 +506,9 @@ class BatchPrefillWithPagedKVCacheWrapper:
         pass
 
     def _device_plan(self, total_qo: int) -> None:
-        what = type(self).__name__ + ".plan"
-        _lib.check(self._plan_call(total_qo), what)
-        _after(what)
+        rc = self._plan_call(total_qo)
+        if rc or _CHECK:
+            self._report(rc, ".plan")
         self._plan_total = total_qo
         self._needs_device_plan = False
 
@@ -536,10 +542,12 @@ class BatchPrefillWithPagedKVCacheWrapper:
             lse = torch.empty((total_qo, self._hq), dtype=torch.float32, device=q.device)
         scale = self._sm_scale if self._sm_scale is not None else 1.0 / math.sqrt(self._d)
         scale *= _check_scales(q_scale, k_scale, v_scale)
-        what = type(self).__name__ + ".run"
-        _lib.check(self._run_call(q, qsn, qsh, desc, total_qo, float(scale), out, lse), what)
-        _after(what)
+        rc = self._run_call(q, qsn, qsh, desc, total_qo, float(scale), out, lse)
+        if rc or _CHECK:
+            self._report(rc, ".run")
         return (out, lse) if return_lse else out
+
+    _report = BatchDecodeWithPagedKVCacheWrapper._report
 
     def _run_call(self, q, qsn, qsh, desc, total_qo, scale, out, lse) -> int:
         return _lib.load().pa_prefill_run(
