@@ -194,16 +194,19 @@ __global__ void __launch_bounds__(kWindowPlanThreads)
   const int ctas = gridDim.x - 1, c = blockIdx.x - 1;
   const int b0 = static_cast<int>(static_cast<int64_t>(batch) * c / ctas);
   const int b1 = static_cast<int>(static_cast<int64_t>(batch) * (c + 1) / ctas);
-  int sum = 0;
+  // (64 bits: the rows of a malformed table may claim the same entries again
+  // and again)
+  __shared__ int64_t s_sum[32];
+  int64_t at = 0;
   for (int b = tid; b < b0; b += kWindowPlanThreads)
-    sum += window_row(kv_indptr, last_len, b, num_indices, page_size, window, sinks).visible;
+    at += window_row(kv_indptr, last_len, b, num_indices, page_size, window, sinks).visible;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  if (lane == 0) s_warp[wid] = sum;
+  for (int off = 16; off > 0; off >>= 1) at += __shfl_xor_sync(0xffffffffu, at, off);
+  if (lane == 0) s_sum[wid] = at;
   __syncthreads();
-  int at = 0;
+  at = 0;
 #pragma unroll
-  for (int w = 0; w < 32; ++w) at += s_warp[w];
+  for (int w = 0; w < 32; ++w) at += s_sum[w];
   // the range's rows, kWindowRows at a time, read by a thread each
   __shared__ int4 s_row[kWindowRows];  // {first table entry, visible pages, sink pages, shift}
   for (int g = b0; g < b1; g += kWindowRows) {

@@ -402,6 +402,23 @@ def test_wrong_tables_are_reported(fi, lir):
         w.run(pr.q.to(DEV), pr.device_pool())
 
 
+def test_rows_that_claim_the_same_entries_again_are_reported(fi, lir):
+    """The visible pages of such a table add up past 32 bits."""
+    n, rows = 1 << 20, 6000
+    indptr = np.zeros(rows + 1, dtype=np.int64)
+    indptr[1::2] = n
+    buf = torch.full((96 << 20,), 7, dtype=torch.uint8, device=DEV)
+    w = fi.BatchDecodeWithSlidingWindowWrapper(buf[32 << 20:64 << 20], "HND", window_left=HUGE)
+    fi._CHECK, saved = False, fi._CHECK
+    try:
+        w.plan(_t(indptr), _t(np.zeros(n)), _t(np.full(rows, P)), 8, 2, 64, P,
+               q_data_type=torch.bfloat16)
+        assert lir._lib.device_status() == lir._lib.PA_ERR_DEVICE_CHECK
+    finally:
+        fi._CHECK = saved
+    assert (buf[:32 << 20] == 7).all() and (buf[64 << 20:] == 7).all()
+
+
 def test_plans_are_not_exchanged(fi):
     """A full plan's workspace is not a window plan's, and the other way round."""
     pr = _decode_problem([100, 50], 8, 2, 64, 20, 0, seed=62, evict=False, poison=False)
