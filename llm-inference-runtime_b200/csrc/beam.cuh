@@ -41,6 +41,11 @@ constexpr int kBeamMany = 128;  // threads at the threshold: many logits are equ
 constexpr int kBeamStep = 2;    // vectors of a thread taken together
 constexpr int kBeamRing = 4;    // such steps in flight
 constexpr float kBeamSlack = 5.f;
+// Logits beyond this are no reference for a sum of 2^(x log2(e) - off): up to
+// here off's rounding (which the sum carries) is at most 64, further out the
+// sum may overflow. fp32 steps there are 128, so such a low logit adds nothing
+// beside any that is not.
+constexpr float kBeamHuge = 1.4e9f;
 constexpr int kBeamRingBytes = kBeamRing * kBeamStep * kBeamThreads * 16;
 static_assert(kBeamRingBytes >= kBeamCap * 8, "the ring holds the candidates at the end");
 
@@ -302,11 +307,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
       second = best;
       best = m;
       best_step = step;
-      // (logits masked by the type's lowest value are no reference: their sum
-      // is 0 beside any other's)
-      if (m > ref + kBeamSlack && m > -1e30f) {
+      if (m > ref + kBeamSlack && m > -kBeamHuge) {
         const float off = m * kLog2e;
-        my_sum *= ex2(my_off - off);  // (0 before the first finite logit)
+        if (ref != -INFINITY) my_sum *= ex2(my_off - off);  // (before that it is 0 or NaN)
         ref = m;
         my_off = off;
       }
@@ -375,7 +378,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
   // this chunk's sum of 2^(x log2(e) - off), off = m log2(e) rounded: the join
   // takes the same off, so its rounding cancels
   const float off = m * kLog2e;
-  const bool huge = fabsf(m) > 1e30f;  // the product may overflow; x - m does as well there
+  const bool huge = fabsf(m) >= kBeamHuge;  // x - m serves there
   if (m == -INFINITY || best == -INFINITY) {
     my_sum = 0.0;
   } else if (huge || !(my_sum < 1e30)) {
@@ -393,9 +396,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
           my_sum += ex2(huge ? (f - m) * kLog2e : fmaf(f, kLog2e, -off));
         }
     }
-  } else {
+  } else if (ref != -INFINITY) {
     my_sum *= ex2(my_off - off);
-  }
+  }  // else: 0, nothing but masked logits
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) my_sum += __shfl_xor_sync(0xffffffffu, my_sum, o);
   if (lane == 0) s_sum[wid] = my_sum;

@@ -148,6 +148,22 @@ def test_masked_logits(beam, dtype):
     check(beam, logits, scores, 16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("mask", ["lowest", -1e30, -1e20, -1e12, -3e9, -1e9, -math.inf])
+def test_low_logits_among_masked_ones(beam, dtype, mask):
+    """Log probabilities far below zero, most tokens masked: whole threads,
+    steps and chunks hold masked logits only."""
+    logits, scores = _random(3, 2, 30000, torch.float32, 19)
+    logits -= 300
+    g = torch.Generator().manual_seed(20)
+    keep = (torch.rand(logits.shape, generator=g) < 0.002).to(DEV)
+    keep[1, :, 4096:] = False
+    keep[2, 1] = False
+    low = torch.finfo(dtype).min
+    value = low if mask == "lowest" else max(mask, low) if math.isfinite(mask) else mask
+    check(beam, logits.masked_fill(~keep, value).to(dtype), scores, 8)
+
+
 def test_beams_that_do_not_continue(beam):
     logits, scores = _random(5, 4, 2500, torch.bfloat16, seed=7)
     scores[0, 1:] = -math.inf           # a first step
