@@ -202,7 +202,9 @@ int pa_fork_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
  *   ref_counts[num_pages]   holders of a page (tables, a prefix cache); 0 = free
  *   block_tables[rows][max_blocks], rows block_table_stride elements apart:
  *     page of tokens [j * page_size, (j + 1) * page_size) of a row, -1 = given back
- *   seq_lens[rows]          tokens a row holds; its entries j < ceil(len / page_size)
+ *   seq_lens[rows]          tokens a row holds; its entries j < ceil(len / page_size).
+ *     Between pa_fork_sequences and the append of the row's token, lengths that
+ *     count this token (len + 1) hold its page too.
  * Errors that only the device sees (a page id outside the pool, a count that
  * falls below zero, no free page left) are recorded as PA_ERR_DEVICE_CHECK and
  * counted in counts[2] where its line says so; sound rows are processed all
@@ -231,7 +233,7 @@ int pa_release_pages(int32_t* block_tables, int64_t block_table_stride, int32_t 
  * taken lowest number first, by ascending r. Entries past the row's are -1.
  * counts receives {pages copied, pages taken, rows left without a page (their
  * entry is -1)}. pool, strides and page_bytes as for pa_fork_pages;
- * out_block_tables must not be block_tables; workspace: 3 * num_sequences
+ * out_block_tables must not overlap block_tables; workspace: 3 * num_sequences
  * int32. */
 int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
                       int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,

@@ -83,7 +83,8 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
 
 def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.Tensor,
                      block_tables: torch.Tensor, seq_lens: torch.Tensor,
-                     ref_counts: torch.Tensor) -> Dict[str, torch.Tensor]:
+                     ref_counts: torch.Tensor, kv_layout: str = "HND"
+                     ) -> Dict[str, torch.Tensor]:
     """One step of beam search: each request's beams are replaced by its
     ``beams`` best continuations and their cache follows.
 
@@ -91,12 +92,14 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.
     request b. Returns scores, parents and tokens [batch, beams] and the new
     block_tables, seq_lens and counts (``pages.fork_sequences``): every beam
     owns the page that its token, to be fed to the model next, is appended
-    to, at position seq_lens[r]."""
+    to, at position seq_lens[r] (the lengths to pass to the next step are these
+    plus one)."""
     batch, beams = scores.shape
     if seq_lens.numel() != batch * beams:
         raise ValueError("block_tables must hold one row per beam of each request")
     best, parents, tokens = beam_search_select(logits, scores, beams)
     tables, lens, counts = pages.fork_sequences(kv_pool, block_tables, seq_lens,
-                                                parents.view(-1), ref_counts)
+                                                parents.view(-1), ref_counts,
+                                                kv_layout=kv_layout)
     return {"scores": best, "parents": parents, "tokens": tokens, "block_tables": tables,
             "seq_lens": lens, "counts": counts}

@@ -8,7 +8,11 @@ step that reorders beams or gives pages back can be captured in a CUDA graph:
 * ``ref_counts`` [pages]: holders of a page (tables, a prefix cache); 0 = free
 * ``block_tables`` [sequences, max_blocks]: page of tokens [16 j, 16 j + 16)
   of a sequence, -1 where it was given back
-* ``seq_lens`` [sequences]: tokens a sequence holds
+* ``seq_lens`` [sequences]: tokens a sequence holds; its pages are the first
+  ceil(seq_len / 16) entries, and what lies behind them is not read. Between a
+  fork and the append of its token the page of that token is held too: a call
+  there counts it (``free_sequences(tables, seq_lens + 1, refs)``,
+  ``compact_pages(pool, tables, seq_lens + 1, refs)``).
 
 Each call returns ``counts``, an int32 device tensor of three; its last entry
 counts what could not be done (it stays 0 in a sound step), which is also
@@ -56,12 +60,19 @@ def _row_stride(t: torch.Tensor) -> int:
     return max(t.stride(0), t.size(1))
 
 
+def _page_size(kv_pool: torch.Tensor, kv_layout: str) -> int:
+    if kv_layout not in ("HND", "NHD"):
+        raise ValueError(f"kv_layout must be 'HND' or 'NHD', not {kv_layout!r}")
+    return kv_pool.size(-2 if kv_layout == "HND" else -3)
+
+
 def _pool(kv_pool: torch.Tensor, ref_counts: torch.Tensor):
     """(pointer, layer stride, layers, page stride, page bytes, pages) in bytes
     of the engine's pool [L, N, 2, H_kv, P, D] or one layer of it."""
     pool = kv_pool if kv_pool.dim() == 6 else kv_pool.unsqueeze(0)
     if pool.dim() != 6 or not pool.is_cuda:
-        raise ValueError("kv_pool must be [L, N, 2, H_kv, P, D] (or one layer) on the GPU")
+        raise ValueError("kv_pool must be [L, N, 2, H_kv, P, D], for NHD [L, N, 2, P, H_kv, D] "
+                         "(or one layer), on the GPU")
     if pool.device != ref_counts.device:
         raise ValueError("kv_pool and ref_counts must be on one GPU")
     if pool.size(1) != ref_counts.numel():
@@ -119,7 +130,7 @@ def free_sequences(block_tables: torch.Tensor, seq_lens: torch.Tensor, ref_count
 
 def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                    parents: torch.Tensor, ref_counts: torch.Tensor,
-                   out: Optional[torch.Tensor] = None
+                   out: Optional[torch.Tensor] = None, kv_layout: str = "HND"
                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Sequence r continues sequence ``parents[r]``: beam search's reordering
     of states, or several samples of one prompt. Returns (block_tables,
@@ -133,7 +144,11 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
     free page for the others. Sequences that nobody continues give up their
     pages. Free pages are those with count 0, taken lowest number first.
     counts: pages copied, pages taken, sequences left without a page (their
-    entry is -1: the pool is full, or the table has no room)."""
+    entry is -1: the pool is full, or the table has no room).
+
+    A sequence's token is appended (at position seq_lens[r], which then grows
+    by one) before it is forked again. ``out`` receives the new tables, for
+    example the other half of a double buffer."""
     device = _state(block_tables, seq_lens, ref_counts)
     _on_gpu_i32(parents, "parents", 1)
     if parents.numel() != seq_lens.numel() or parents.device != device:
@@ -146,8 +161,10 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
         raise ValueError("out must have block_tables' shape and device")
     else:
         _on_gpu_i32(out, "out", 2)
-        if rows and width and (out.untyped_storage().data_ptr()
-                               == block_tables.untyped_storage().data_ptr()):
+        span = 4 * ((rows - 1) * _row_stride(block_tables) + width)
+        out_span = 4 * ((rows - 1) * _row_stride(out) + width)
+        if rows and width and (out.data_ptr() < block_tables.data_ptr() + span
+                               and block_tables.data_ptr() < out.data_ptr() + out_span):
             raise ValueError("out must not share memory with block_tables")
     # lengths and counts that go back, then the kernels' scratch
     ints = torch.empty(4 * rows + 3, dtype=torch.int32, device=device)
@@ -156,14 +173,15 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
         _lib.check(_lib.load().pa_fork_sequences(
             ptr, layer_stride, layers, page_stride, page_bytes, pages, block_tables.data_ptr(),
             _row_stride(block_tables), width, seq_lens.data_ptr(), parents.data_ptr(), rows,
-            kv_pool.size(-2), ref_counts.data_ptr(), out.data_ptr(), _row_stride(out),
+            _page_size(kv_pool, kv_layout), ref_counts.data_ptr(), out.data_ptr(), _row_stride(out),
             lens.data_ptr(), counts.data_ptr(), scratch, _stream()), "fork_sequences")
         _after("fork_sequences")
     return out, lens, counts
 
 
 def compact_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
-                  ref_counts: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+                  ref_counts: torch.Tensor, kv_layout: str = "HND"
+                  ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Moves the live pages (count > 0) to the front of the pool, in place:
     with n of them, the k-th live page at or past n goes to the k-th free page
     before n (all layers); ``ref_counts`` and the entries of ``block_tables``
@@ -180,7 +198,7 @@ def compact_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: t
         _lib.check(_lib.load().pa_compact_pages(
             ptr, layer_stride, layers, page_stride, page_bytes, pages, block_tables.data_ptr(),
             _row_stride(block_tables), block_tables.size(1), seq_lens.data_ptr(),
-            seq_lens.numel(), kv_pool.size(-2), ref_counts.data_ptr(), remap.data_ptr(),
-            counts.data_ptr(), scratch.data_ptr(), _stream()), "compact_pages")
+            seq_lens.numel(), _page_size(kv_pool, kv_layout), ref_counts.data_ptr(),
+            remap.data_ptr(), counts.data_ptr(), scratch.data_ptr(), _stream()), "compact_pages")
         _after("compact_pages")
     return remap, counts

@@ -288,6 +288,71 @@ def test_fork_pool_shapes(pages):
     assert torch.equal(_bits(big[:, 1::2]), _bits(before[:, 1::2]))
 
 
+def test_nhd_pools(pages):
+    """A page is a block of bytes in either layout; its tokens are counted
+    along the layout's own dimension."""
+    tables, lens, refs, rng = _random_state(78, 12, 200, spare=24)
+    parents = rng.randint(0, 12, 12)
+    pool = _pool(len(refs), 2, 8, 64).permute(0, 1, 2, 4, 3, 5).contiguous()
+    want_t, want_l, want_r, want_c, copies = plain_fork(tables, lens, refs, parents)
+    want_pool, c = _copied(pool, copies), _i32(refs)
+    t, n, counts = pages.fork_sequences(pool, _i32(tables), _i32(lens), _i32(parents), c,
+                                        kv_layout="NHD")
+    assert np.array_equal(t.cpu().numpy(), want_t) and counts.tolist() == want_c
+    assert np.array_equal(c.cpu().numpy(), want_r) and np.array_equal(n.cpu().numpy(), want_l)
+    assert torch.equal(_bits(pool), _bits(want_pool))
+    want_t, want_r, want_m, want_c, copies = plain_compact(want_t, want_l + 1, want_r)
+    want_pool = _copied(pool, copies)
+    remap, counts = pages.compact_pages(pool, t, n + 1, c, kv_layout="NHD")
+    assert np.array_equal(t.cpu().numpy(), want_t) and counts.tolist() == want_c
+    assert np.array_equal(c.cpu().numpy(), want_r) and torch.equal(_bits(pool), _bits(want_pool))
+    assert np.array_equal(remap.cpu().numpy(), want_m)
+    for call in (lambda: pages.fork_sequences(pool, t, n, n, c, kv_layout="DNH"),
+                 lambda: pages.compact_pages(pool, t, n, c, "hnd")):
+        with pytest.raises(ValueError, match="kv_layout"):
+            call()
+
+
+def test_fork_between_the_halves_of_one_buffer(pages):
+    tables, lens, refs, rng = _random_state(79, 10, 100, spare=30)
+    parents = rng.randint(0, 10, 10)
+    both = torch.full((2,) + tables.shape, -7, dtype=torch.int32, device=DEV)
+    both[1] = _i32(tables)
+    pool, c = _pool(len(refs), 1), _i32(refs)
+    t, _, counts = pages.fork_sequences(pool, both[1], _i32(lens), _i32(parents), c, out=both[0])
+    want_t, _, want_r, want_c, _ = plain_fork(tables, lens, refs, parents)
+    assert t.data_ptr() == both.data_ptr() and np.array_equal(both[0].cpu().numpy(), want_t)
+    assert np.array_equal(both[1].cpu().numpy(), tables) and counts.tolist() == want_c
+    flat = both.view(-1, tables.shape[1])
+    for k in (0, 2, 4, 5, 10):
+        with pytest.raises(ValueError, match="share memory"):
+            pages.fork_sequences(pool, flat[5:15], _i32(lens), _i32(parents), c,
+                                 out=flat[k:k + 10])
+    assert np.array_equal(c.cpu().numpy(), want_r)
+
+
+@pytest.mark.parametrize("length", [0, 16, 31, 32, 33])
+def test_free_and_compact_between_a_fork_and_its_append(pages, length):
+    """The page of the token to come is held once lengths count that token."""
+    n = _held(length)
+    tables = np.full((3, n + 2), -1, dtype=np.int64)
+    tables[:, :n] = np.arange(n) + 20
+    refs = np.zeros(40, dtype=np.int64)
+    refs[20:20 + n] = 3
+    refs[0] = 1  # held elsewhere
+    t, ln, c, pool = _check_fork(pages, tables, np.full(3, length), refs, np.array([1, 1, 2]))
+    own = t.cpu().numpy()[:, length // P]
+    assert len(set(own.tolist())) == 3 and (own >= 0).all()
+    fresh = pool.clone()
+    pages.compact_pages(pool, t, ln + 1, c)
+    moved = t.cpu().numpy()[:, length // P]
+    for a, b in zip(own, moved):
+        assert torch.equal(_bits(pool[:, b]), _bits(fresh[:, a]))
+    assert c[moved.tolist()].tolist() == [1] * 3
+    pages.free_sequences(t, ln + 1, c)
+    assert c.sum() == 1 and (t == -1).all()
+
+
 def test_fork_with_no_page_left(pages):
     tables = np.array([[0, 1, -1], [2, 3, -1], [4, 5, 6]])
     lens, refs = np.array([20, 32, 48]), np.ones(7, dtype=np.int64)
