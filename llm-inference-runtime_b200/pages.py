@@ -34,7 +34,7 @@ def _on_gpu_i32(t: torch.Tensor, name: str, dim: int) -> torch.Tensor:
         raise TypeError(f"{name} must be int32")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
-    if t.dim() != dim or (t.numel() > 0 and t.stride(-1) != 1):
+    if t.dim() != dim or (t.stride()[-1] != 1 and t.numel() > 0):
         raise ValueError(f"{name} must be {dim}-D with contiguous entries")
     return t
 
@@ -55,9 +55,13 @@ def _state(block_tables, seq_lens, ref_counts) -> torch.device:
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between rows; rows of their own (a broadcast table has one)."""
-    if t.size(0) > 1 and t.stride(0) < t.size(1):
+    rows, width = t.shape
+    stride = t.stride()[0]
+    if stride >= width:
+        return stride
+    if rows > 1:
         raise ValueError("the rows of block_tables must not overlap")
-    return max(t.stride(0), t.size(1))
+    return width
 
 
 def _page_size(kv_pool: torch.Tensor, kv_layout: str) -> int:
@@ -93,10 +97,10 @@ def _pool(kv_pool: torch.Tensor, ref_counts: torch.Tensor):
 
 def _release(what, block_tables, seq_lens, ref_counts, page_size, window_left, sinks):
     device = _state(block_tables, seq_lens, ref_counts)
-    counts = torch.empty(3, dtype=torch.int32, device=device)
+    counts = ref_counts.new_empty(3)
     with _device_guard(device):
         _lib.check(_lib.load().pa_release_pages(
-            block_tables.data_ptr(), _row_stride(block_tables), block_tables.size(1),
+            block_tables.data_ptr(), _row_stride(block_tables), block_tables.shape[1],
             seq_lens.data_ptr(), seq_lens.numel(), int(page_size), window_left, sinks,
             ref_counts.data_ptr(), ref_counts.numel(), counts.data_ptr(), _stream()), what)
         _after(what)
@@ -156,7 +160,7 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
     ptr, layer_stride, layers, page_stride, page_bytes, pages = _pool(kv_pool, ref_counts)
     rows, width = block_tables.shape
     if out is None:
-        out = torch.empty((rows, width), dtype=torch.int32, device=device)
+        out = block_tables.new_empty((rows, width))
     elif out.shape != block_tables.shape or out.device != device:
         raise ValueError("out must have block_tables' shape and device")
     else:
@@ -167,14 +171,13 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
                                and block_tables.data_ptr() < out.data_ptr() + out_span):
             raise ValueError("out must not share memory with block_tables")
     # lengths and counts that go back, then the kernels' scratch
-    ints = torch.empty(4 * rows + 3, dtype=torch.int32, device=device)
-    lens, counts, scratch = ints[:rows], ints[rows:rows + 3], ints.data_ptr() + 4 * (rows + 3)
+    lens, counts, scratch = ref_counts.new_empty(4 * rows + 3).split_with_sizes((rows, 3, 3 * rows))
     with _device_guard(device):
         _lib.check(_lib.load().pa_fork_sequences(
             ptr, layer_stride, layers, page_stride, page_bytes, pages, block_tables.data_ptr(),
             _row_stride(block_tables), width, seq_lens.data_ptr(), parents.data_ptr(), rows,
             _page_size(kv_pool, kv_layout), ref_counts.data_ptr(), out.data_ptr(), _row_stride(out),
-            lens.data_ptr(), counts.data_ptr(), scratch, _stream()), "fork_sequences")
+            lens.data_ptr(), counts.data_ptr(), scratch.data_ptr(), _stream()), "fork_sequences")
         _after("fork_sequences")
     return out, lens, counts
 
@@ -191,9 +194,8 @@ def compact_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: t
     nobody holds; they stay)."""
     device = _state(block_tables, seq_lens, ref_counts)
     ptr, layer_stride, layers, page_stride, page_bytes, pages = _pool(kv_pool, ref_counts)
-    remap = torch.empty(pages, dtype=torch.int32, device=device)
-    counts = torch.empty(3, dtype=torch.int32, device=device)
-    scratch = torch.empty(pages + 2, dtype=torch.int32, device=device)
+    remap, counts = ref_counts.new_empty(pages), ref_counts.new_empty(3)
+    scratch = ref_counts.new_empty(pages + 2)
     with _device_guard(device):
         _lib.check(_lib.load().pa_compact_pages(
             ptr, layer_stride, layers, page_stride, page_bytes, pages, block_tables.data_ptr(),
