@@ -743,8 +743,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     uint32_t kt = 0;  // running tile count = running step count
     for (int it = 0;; ++it) {
     int ntiles, kv_len, lim;
-    int hole_lo = 0, hole_hi = 0;    // hidden from this row
-    int ihole_lo = 0, ihole_hi = 0;  // hidden from every row of the item
+    // keys [sinks, hole_hi) are hidden from this row, and some before
+    // ihole_hi from every row of the item
+    [[maybe_unused]] int hole_hi = 0, ihole_hi = 0;
     {
       const PfItem w = wait_item(it);
       ntiles = w.ntiles;
@@ -753,11 +754,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       lim = p.causal ? min(qpos + 1, kv_len) : kv_len;
       if constexpr (kWindow) {
         const int skip = w.shift * kPage;
-        kv_len -= skip;
         lim -= skip;
-        hole_lo = p.sinks;
         hole_hi = max(qpos - p.window, 0) - skip;
-        ihole_lo = w.hole_lo;
         ihole_hi = w.hole_hi;
       }
     }
@@ -783,17 +781,25 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       tmem_wait_ld();
       const int key0 = j * kPfKeys;
       if constexpr (kWindow) {
-        // hidden: columns >= lim - key0, and columns [a, b)
-        const int a = hole_lo - key0, b = hole_hi - key0, e = lim - key0;
-        if (!__all_sync(0xffffffffu, e >= kPfKeys)) {
+        // Hidden: columns >= e, and columns [a, b). Both as one bit mask per
+        // 32 columns, and only where a row of the warp hides some of them: a
+        // tile's 128 comparisons with each end took 147 us where this takes
+        // 141 (16 chunks of 512 rows, window 1024, 32 heads of 128).
+        const int a = p.sinks - key0, b = hole_hi - key0, e = lim - key0;
+        if (!__all_sync(0xffffffffu, e >= kPfKeys && b <= 0)) {
+          auto below = [](int x) {  // bits 0 .. x - 1
+            return __funnelshift_lc(0u, 1u, static_cast<uint32_t>(min(max(x, 0), 32))) - 1u;
+          };
 #pragma unroll
-          for (int c = 0; c < kPfKeys; ++c)
-            if (c >= e) s[c] = -INFINITY;
-        }
-        if (!__all_sync(0xffffffffu, a >= kPfKeys || b <= 0 || a >= b)) {
+          for (int ch = 0; ch < kPfKeys / 32; ++ch) {
+            const uint32_t seen =
+                below(e - 32 * ch) & ~(below(b - 32 * ch) & ~below(a - 32 * ch));
+            if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
-          for (int c = 0; c < kPfKeys; ++c)
-            if (c >= a && c < b) s[c] = -INFINITY;
+              for (int c = 0; c < 32; ++c)
+                if (!(seen & (1u << c))) s[32 * ch + c] = -INFINITY;
+            }
+          }
         }
       } else if (!__all_sync(0xffffffffu, key0 + kPfKeys <= lim)) {
 #pragma unroll
@@ -851,11 +857,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       // The last tile may hold keys past kv_len (stale slots, pages never
       // loaded): tile 0's warpgroup zeroes those V rows before its PV, which
       // precedes tile 1's PV on the tensor pipe.
-      bool clear = j == ntiles - 1 && key0 + kPfKeys > kv_len;
-      // the same for keys that the window hides from the whole item: their
-      // tokens must not reach O, whatever they are
-      if constexpr (kWindow)
-        clear = clear || (ihole_lo < ihole_hi && ihole_lo < key0 + kPfKeys && ihole_hi > key0);
+      bool clear = j == ntiles - 1;
+      // (the same for keys that the window hides from the whole item: their
+      // tokens must not reach O, whatever they are; its limits are read again
+      // where they may matter, registers being short here)
+      if constexpr (kWindow) {
+        clear = clear || ihole_hi > key0;
+      } else {
+        clear = clear && key0 + kPfKeys > kv_len;
+      }
       if (t == 0 && clear) {
         const int st = g % S;
         if (!mbar_wait_warp(&v_full[st], (g / S) & 1)) {
@@ -863,8 +873,11 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           break;
         }
         bool drop = key0 + r >= kv_len;
-        if constexpr (kWindow)
-          drop = drop || (key0 + r >= ihole_lo && key0 + r < ihole_hi);
+        if constexpr (kWindow) {
+          const PfItem& w = slots[it % 3];
+          drop = key0 + r >= w.kv_len - w.shift * kPage ||
+                 (key0 + r >= w.hole_lo && key0 + r < w.hole_hi);
+        }
         if (drop) {
 #pragma unroll
           for (int pn = 0; pn < C::kPanels; ++pn)
