@@ -13,13 +13,15 @@
 // request.
 //
 // Chunk pass: a CTA streams its chunk once, two 16-byte vectors a thread at a
-// time with six more on their way; each thread keeps its own maximum and
+// time with four more on their way; each thread keeps its own maximum and
 // the sum relative to it, so nothing waits on another thread until the end.
 // Of the 256 threads' maxima each warp's four best are looked at; the K-th of
 // those 32 is a threshold that at least K logits reach and few others do. The
-// threads whose maximum reaches it (about K of 256) have the step that holds it
-// read again, a word per lane (all their logits if another step reaches it
-// too), and what passes is ranked by counting. Many threads
+// threads whose maximum reaches it (about K of 256) have the steps that hold
+// their two largest maxima searched, which every thread keeps in shared memory
+// (all their logits are read again if a third step reaches it too), and what
+// passes is ranked by counting. (Reading the step again instead of keeping it
+// took 3 us of a CTA's 19, now 0.9.) Many threads
 // reach it only when many logits are equal to it (masked or constant rows):
 // then the ones above it and, in index order, as many equal ones as are missing
 // are taken. If more than kBeamCap lie above it (a layout against the threads'
@@ -31,6 +33,7 @@
 namespace pa {
 
 constexpr int kBeamThreads = 256;
+constexpr int kBeamCtas = 5;    // per SM, of 40 KB (4 with a deeper ring: 37.5 for 37.2 us)
 constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamMaxK = 32;   // the threshold looks at 32 maxima
 constexpr int kBeamMaxBeams = 256;      // JoinKey's 8 bits
@@ -39,7 +42,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kBeamCap = 1024;  // elements ranked by counting
 constexpr int kBeamMany = 128;  // threads at the threshold: many logits are equal to it
 constexpr int kBeamStep = 2;    // vectors of a thread taken together
-constexpr int kBeamRing = 4;    // such steps in flight
+constexpr int kBeamRing = 3;    // such steps in flight
 constexpr float kBeamSlack = 5.f;
 // Logits beyond this are no reference for a sum of 2^(x log2(e) - off): up to
 // here off's rounding (which the sum carries) is at most 64, further out the
@@ -47,6 +50,7 @@ constexpr float kBeamSlack = 5.f;
 // beside any that is not.
 constexpr float kBeamHuge = 1.4e9f;
 constexpr int kBeamRingBytes = kBeamRing * kBeamStep * kBeamThreads * 16;
+constexpr int kBeamSmem = kBeamRingBytes + 2 * kBeamStep * kBeamThreads * 16;  // and two steps kept
 static_assert(kBeamRingBytes >= kBeamCap * 8, "the ring holds the candidates at the end");
 
 struct BeamParams {
@@ -235,7 +239,7 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p, int bytes) {
 // HBM). NaN needs no instruction of its own: maxima and comparisons pass over
 // it, and a thread whose sum is not finite adds its logits up again, cleaned.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kBeamThreads, kBeamCtas) beam_chunk_kernel(const BeamParams p) {
   using W = BeamWord<T>;
   constexpr int N = 16 / sizeof(T);
   constexpr int kRow = kBeamThreads * N;  // logits per vector of all threads
@@ -245,13 +249,15 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
   __shared__ int s_warp[kBeamWarps];
   extern __shared__ uint4 ring[];  // kBeamRing steps
   uint64_t* const s_cand = reinterpret_cast<uint64_t*>(ring);  // [kBeamCap], once they are taken
-  __shared__ int s_who[kBeamThreads];
+  uint4* const keep = ring + kBeamRing * kBeamStep * kBeamThreads;  // two steps of each thread
+  __shared__ int s_who[2 * kBeamMany];
   __shared__ int s_n, s_one, s_all;
   griddep_wait();
   griddep_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int chunk = blockIdx.x, w = blockIdx.y, b = blockIdx.z;
-  const int64_t part = (static_cast<int64_t>(b) * p.beams + w) * p.chunks + chunk;
+  // rows first: the rows' last chunks, which may be shorter, start last
+  const int b = blockIdx.x / p.beams, w = blockIdx.x - b * p.beams, chunk = blockIdx.y;
+  const int64_t part = static_cast<int64_t>(blockIdx.x) * p.chunks + chunk;
   const T* x = static_cast<const T*>(p.logits) + b * p.stride_b + w * p.stride_w;
   const int base = chunk * p.chunk_vectors * kRow, K = p.k;
   const int vectors = min(p.chunk_vectors, (p.vocab - base + kRow - 1) / kRow);  // > 0
@@ -286,8 +292,15 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
   // the sum one rounding of ex2)
   float ref = -INFINITY, my_off = 0.f;
   double my_sum = 0.0;
-  int best_step = 0;       // where `best` is
-  float second = -INFINITY;  // the largest logit of the other steps
+  // The two steps with the largest maxima are kept, slot of `best` and the
+  // other one, and the largest logit of all others: nearly every logit that
+  // the threshold lets through is then at hand.
+  float second = -INFINITY, third = -INFINITY;
+  int best_step = 0, second_step = 0, slot = 0;
+  auto save = [&](const uint4 (&in)[kBeamStep], int to) {
+#pragma unroll
+    for (int u = 0; u < kBeamStep; ++u) keep[(to * kBeamStep + u) * kBeamThreads + tid] = in[u];
+  };
   auto take = [&](const uint4 (&in)[kBeamStep], int step) {
     uint32_t v[kBeamStep][4];
 #pragma unroll
@@ -304,17 +317,26 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
       for (int q = 0; q < 4; ++q) m2 = W::max2(m2, v[u][q]);
     const float m = W::N == 2 ? fmaxf(W::at(m2, 0), W::at(m2, 1)) : W::at(m2, 0);
     if (m > best) {
+      third = second;
       second = best;
       best = m;
+      second_step = best_step;
       best_step = step;
+      slot ^= 1;
+      save(in, slot);
       if (m > ref + kBeamSlack && m > -kBeamHuge) {
         const float off = m * kLog2e;
         if (ref != -INFINITY) my_sum *= ex2(my_off - off);  // (before that it is 0 or NaN)
         ref = m;
         my_off = off;
       }
+    } else if (m > second) {
+      third = second;
+      second = m;
+      second_step = step;
+      save(in, slot ^ 1);
     } else {
-      second = fmaxf(second, m);
+      third = fmaxf(third, m);
     }
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -366,13 +388,19 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
   uint32_t top;
   const uint32_t least = block_threshold(mine, K, s_four, lane, wid, &top);
   const float m = order_value(top);  // the chunk is not empty
-  // Threads at the threshold: usually with one step's logits only, which are
-  // listed from the front, otherwise from the back. (Both counters were set
+  // Threads at the threshold: their kept steps that reach it are listed, or,
+  // should a third one reach it too, the thread. (Both counters were set
   // before the barrier above.)
   if (mine >= least && mine != 0) {
-    const bool one = order_bits(fminf(second, W::kMost) + 0.f) < least;
-    const int at = one ? atomicAdd(&s_one, 1) : kBeamThreads - 1 - atomicAdd(&s_all, 1);
-    s_who[at] = best_step << 8 | tid;
+    if (order_bits(fminf(third, W::kMost) + 0.f) >= least) {
+      const int at = atomicAdd(&s_all, 1);
+      if (at < kBeamMany) s_who[kBeamMany + at] = tid;
+    } else {
+      const bool two = order_bits(fminf(second, W::kMost) + 0.f) >= least;
+      const int at = atomicAdd(&s_one, two ? 2 : 1);
+      if (at < kBeamMany) s_who[at] = best_step << 9 | slot << 8 | tid;
+      if (two && at + 1 < kBeamMany) s_who[at + 1] = second_step << 9 | (slot ^ 1) << 8 | tid;
+    }
   }
 
   // this chunk's sum of 2^(x log2(e) - off), off = m log2(e) rounded: the join
@@ -410,36 +438,32 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_chunk_kernel(const BeamP
     return base + (i * kBeamThreads + tid) * N + q * W::N + e;
   };
   const int ones = s_one, alls = s_all;
-  const bool many = ones + alls > kBeamMany || least <= order_bits(-INFINITY);
-  // word `word` of a thread's vectors
-  auto look = [&](int thread, int word) {
-    const int i = word >> 2, at = base + (i * kBeamThreads + thread) * N + (word & 3) * W::N;
-    if (i < whole) {  // both of a word at once; mostly neither passes
-      const uint32_t v2 = W::clean(__ldg(reinterpret_cast<const uint32_t*>(x + at)));
-      const float f = W::N == 2 ? fmaxf(W::at(v2, 0), W::at(v2, 1)) : W::at(v2, 0);
-      if (order_bits(f + 0.f) < least) return;
-    }
-#pragma unroll
-    for (int e = 0; e < W::N; ++e) {
-      if (at + e >= p.vocab) continue;
-      const float raw = static_cast<float>(__ldg(x + at + e));
-      const float f = fminf(raw, W::kMost) + 0.f;
-      if (raw == raw && order_bits(f) >= least) {
-        const int n = atomicAdd(&s_n, 1);
-        if (n < kBeamCap) s_cand[n] = beam_key(f, at + e);
-      }
+  const bool many = ones > kBeamMany || alls > kBeamMany || least <= order_bits(-INFINITY);
+  // one logit: a candidate if it reaches the threshold (NaN does not)
+  auto look = [&](float raw, int at) {
+    const float f = fminf(raw, W::kMost) + 0.f;
+    if (raw == raw && at < p.vocab && order_bits(f) >= least) {
+      const int n = atomicAdd(&s_n, 1);
+      if (n < kBeamCap) s_cand[n] = beam_key(f, at);
     }
   };
   if (!many) {
     constexpr int kWords = kBeamStep * 4;  // a step's
     for (int k = tid / kWords; k < ones; k += kBeamThreads / kWords) {
-      const int who = s_who[k], word = (who >> 8) * kWords + tid % kWords;
-      if (word < vectors * 4) look(who & 255, word);
+      const int who = s_who[k], thread = who & 255, u = tid % kWords / 4, q = tid % 4;
+      const uint32_t word = reinterpret_cast<const uint32_t*>(
+          keep)[(((who >> 8 & 1) * kBeamStep + u) * kBeamThreads + thread) * 4 + q];
+      const int at =
+          base + (((who >> 9) * kBeamStep + u) * kBeamThreads + thread) * N + q * W::N;
+#pragma unroll
+      for (int e = 0; e < W::N; ++e) look(W::at(word, e), at + e);
     }
+    // (rare: from memory again)
     for (int k = wid; k < alls; k += kBeamWarps)
-#pragma unroll 2
-      for (int word = lane; word < vectors * 4; word += 32)
-        look(s_who[kBeamThreads - 1 - k] & 255, word);
+      for (int i = lane; i < vectors * N; i += 32) {
+        const int at = base + (i / N * kBeamThreads + s_who[kBeamMany + k]) * N + i % N;
+        if (at < p.vocab) look(static_cast<float>(__ldg(x + at)), at);
+      }
   }
   __syncthreads();
   if (tid == 0) {

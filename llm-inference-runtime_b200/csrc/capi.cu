@@ -772,11 +772,14 @@ int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
 namespace {
 
 // How a row is cut: chunks per row, and 16-byte vectors of each thread per
-// chunk. Enough chunks for four CTAs per SM, unless that makes the join's
-// candidates (beams x chunks x k) more than its threads hold: 8 beams of one
-// request over 128256 bf16 logits take 18.1 us in 32 chunks a row, 12.5 in 16
-// and 10.2 in 8; 64 such requests 38.2 us with this target, 45.5 with one CTA
-// per SM and 44.4 with sixteen.
+// chunk (the last one may have fewer). As many chunks as all fit on the GPU at
+// once, unless that makes the join's candidates (beams x chunks x k) more than
+// its threads hold: 8 beams of one request over 128256 bf16 logits take 18.1
+// us in 32 chunks a row, 12.5 in 16 and 10.2 in 8. Where that leaves many
+// places free (few chunks a row) each row gets one more, shorter chunk; these
+// start last and fill the places in turn while the others still run: 64 such
+// requests take 37.9 us with one chunk a row, 37.6 with two halves, 37.3 so;
+// over 50257 tokens 31.0 with halves, 26.7 so.
 struct BeamCut {
   int chunks, vectors;
 };
@@ -786,9 +789,18 @@ BeamCut beam_cut(int dtype, int batch, int beams, int vocab, int k, int sms) {
   const int all = (vocab + row - 1) / row;
   const int64_t rows = std::max<int64_t>(1, static_cast<int64_t>(batch) * beams);
   const int64_t most = std::max<int64_t>(4, kBeamThreads * kBeamHeld / (beams * k));
-  const int64_t want = std::max<int64_t>(1, std::min((4 * sms + rows - 1) / rows, most));
+  const int64_t slots = static_cast<int64_t>(kBeamCtas) * sms;
+  const int64_t full = std::max<int64_t>(1, std::min(slots / rows, most));
   BeamCut c;
-  c.vectors = static_cast<int>(std::max<int64_t>((all + want - 1) / want, kBeamStep));
+  c.vectors = static_cast<int>((all + full - 1) / full);
+  const int64_t spare = slots - full * rows;
+  if (full <= 3 && full < most && spare > 0) {
+    // a chunk is as long as `rounds` short ones, one less than come to a place
+    // (each has its own start and end)
+    const int64_t rounds = std::max<int64_t>(1, (rows + spare - 1) / spare - 1);
+    if (rounds <= 4) c.vectors = static_cast<int>((all * rounds + full * rounds) / (full * rounds + 1));
+  }
+  c.vectors = std::max((c.vectors + kBeamStep - 1) / kBeamStep * kBeamStep, kBeamStep);
   c.chunks = (all + c.vectors - 1) / c.vectors;
   return c;
 }
@@ -871,11 +883,11 @@ int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_s
   p.out_parents = out_parents;
   p.out_tokens = out_tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(cut.chunks, num_beams, batch_size), block(kBeamThreads);
+  const dim3 grid(static_cast<unsigned>(rows), cut.chunks), block(kBeamThreads);
   static std::atomic<uint64_t> done[3];
   auto go = [&](auto kernel, std::atomic<uint64_t>* mask) -> int {
-    if (allow_smem(kernel, kBeamRingBytes, mask, dev) != cudaSuccess) return PA_ERR_CUDA;
-    return launch_chain(kernel, grid, block, kBeamRingBytes, s, p);
+    if (allow_smem(kernel, kBeamSmem, mask, dev) != cudaSuccess) return PA_ERR_CUDA;
+    return launch_chain(kernel, grid, block, kBeamSmem, s, p);
   };
   const int rc = dtype == PA_DTYPE_F32    ? go(beam_chunk_kernel<float>, &done[0])
                  : dtype == PA_DTYPE_BF16 ? go(beam_chunk_kernel<__nv_bfloat16>, &done[1])

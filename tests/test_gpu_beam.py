@@ -148,6 +148,24 @@ def test_masked_logits(beam, dtype):
     check(beam, logits, scores, 16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("apart", [1, 256, 512, 4096])
+@pytest.mark.parametrize("many", [1, 2, 3, 9, 40])
+def test_best_logits_near_one_another(beam, dtype, many, apart):
+    """The best ones sit in one vector, in neighbouring vectors or in several
+    steps of one thread, in ascending and descending order."""
+    logits, scores = _random(2, 3, 50000, dtype, 23)
+    n = 16 // dtype.itemsize
+    for w, start in ((0, 3), (1, 20000), (2, 0)):
+        at = start + torch.arange(many) * (apart * n if apart > 1 else 1)
+        at = at[at < 50000]
+        up = 20 + torch.arange(len(at), dtype=torch.float32)
+        logits[0, w, at] = up.to(dtype).to(DEV)
+        logits[1, w, at] = up.flip(0).to(dtype).to(DEV)
+    check(beam, logits, scores, 8)
+    check(beam, logits, scores, 32)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("mask", ["lowest", -1e30, -1e20, -1e12, -3e9, -1e9, -math.inf])
 def test_low_logits_among_masked_ones(beam, dtype, mask):
