@@ -44,11 +44,6 @@ constexpr int kBeamMany = 128;  // threads at the threshold: many logits are equ
 constexpr int kBeamStep = 2;    // vectors of a thread taken together
 constexpr int kBeamRing = 3;    // such steps in flight
 constexpr float kBeamSlack = 5.f;
-// Logits beyond this are no reference for a sum of 2^(x log2(e) - off): up to
-// here off's rounding (which the sum carries) is at most 64, further out the
-// sum may overflow. fp32 steps there are 128, so such a low logit adds nothing
-// beside any that is not.
-constexpr float kBeamHuge = 1.4e9f;
 constexpr int kBeamRingBytes = kBeamRing * kBeamStep * kBeamThreads * 16;
 constexpr int kBeamSmem = kBeamRingBytes + 2 * kBeamStep * kBeamThreads * 16;  // and two steps kept
 static_assert(kBeamRingBytes >= kBeamCap * 8, "the ring holds the candidates at the end");
@@ -60,8 +55,8 @@ struct BeamParams {
   int64_t score_stride;
   int32_t batch, beams, vocab, k;
   int32_t chunks, chunk_vectors;  // per row; 16-byte vectors of each thread per chunk
-  double* part_off;   // [rows, chunks]: off, about max * log2(e); -inf: nothing finite
-  double* part_sum;   // [rows, chunks]: sum of 2^(x log2(e) - off)
+  double* part_off;   // [rows, chunks]: max * log2(e); -inf: nothing finite
+  double* part_sum;   // [rows, chunks]: sum of exp(x - max)
   uint64_t* part_key;  // [rows, chunks, k]: best first, 0: none
   float* out_scores;  // [batch, k]
   int32_t* out_parents;
@@ -233,8 +228,11 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p, int bytes) {
 // * N and the N - 1 after it whatever the row's alignment, so equal rows give
 // equal sums; places past the row hold -inf.
 //
-// Per logit: half an instruction of packed maxima and four for the sum
-// (unpack, fma, ex2, add). ex2 is the narrowest pipe (16 per
+// Per logit: half an instruction of packed maxima and 3.5 for the sum (unpack,
+// ex2, and subtract, multiply and add for two at a time: 36.9 us where one at
+// a time takes 37.7. x log2(e) - ref log2(e) in one fma took 37.4; its rounding
+// overflows ex2 for huge logits and costs a certain token its log probability
+// of 0). ex2 is the narrowest pipe (16 per
 // SM and cycle: 128256 logits of 512 rows take 14.4 us of it, and 20.1 us of
 // HBM). NaN needs no instruction of its own: maxima and comparisons pass over
 // it, and a thread whose sum is not finite adds its logits up again, cleaned.
@@ -287,10 +285,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) beam_chunk_kernel(con
   const int whole = aligned && !dead ? min(vectors, (p.vocab - base) / kRow) : 0;
   const uint4* src = reinterpret_cast<const uint4*>(x + base) + tid;
   float best = -INFINITY;
-  // the sum of 2^(x log2(e) - my_off), my_off = ref log2(e) rounded; ref
-  // follows the maximum only when it has grown by kBeamSlack (each time costs
-  // the sum one rounding of ex2)
-  float ref = -INFINITY, my_off = 0.f;
+  // the sum of exp(x - ref); ref follows the maximum only when it has grown by
+  // kBeamSlack (each time costs the sum one rounding of ex2), and is 0 before
+  // the first finite logit
+  float ref = 0.f, move = -INFINITY;  // move: where ref follows
   double my_sum = 0.0;
   // The two steps with the largest maxima are kept, slot of `best` and the
   // other one, and the largest logit of all others: nearly every logit that
@@ -324,11 +322,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) beam_chunk_kernel(con
       best_step = step;
       slot ^= 1;
       save(in, slot);
-      if (m > ref + kBeamSlack && m > -kBeamHuge) {
-        const float off = m * kLog2e;
-        if (ref != -INFINITY) my_sum *= ex2(my_off - off);  // (before that it is 0 or NaN)
+      if (m > move) {
+        if (move != -INFINITY) my_sum *= ex2((ref - m) * kLog2e);  // (before that it is 0 or NaN)
         ref = m;
-        my_off = off;
+        move = m + kBeamSlack;
       }
     } else if (m > second) {
       third = second;
@@ -338,15 +335,22 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) beam_chunk_kernel(con
     } else {
       third = fmaxf(third, m);
     }
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    // (two at a time: one word of 16-bit logits, two of fp32)
+    const F32x2 minus_ref(-ref, -ref), scale(kLog2e, kLog2e);
+    F32x2 part[2] = {F32x2(0.f, 0.f), F32x2(0.f, 0.f)};
+    constexpr int kPair = 3 - W::N;  // words of a pair
 #pragma unroll
     for (int u = 0; u < kBeamStep; ++u)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int e = 0; e < W::N; ++e)
-          part[(q * W::N + e) & 3] += ex2(fmaf(W::at(v[u][q], e), kLog2e, -my_off));
-    my_sum += (part[0] + part[1]) + (part[2] + part[3]);
+      for (int q = 0; q < 4; q += kPair) {
+        const F32x2 x(W::at(v[u][q], 0),
+                      W::N == 2 ? W::at(v[u][q], 1) : W::at(v[u][(q + 1) & 3], 0));
+        const F32x2 t = (x + minus_ref) * scale;
+        F32x2& p2 = part[q / kPair & 1];
+        p2 = p2 + F32x2(ex2(t.lo()), ex2(t.hi()));
+      }
+    const F32x2 both = part[0] + part[1];
+    my_sum += both.lo() + both.hi();
   };
   // Steps of whole vectors first, through a ring of shared memory in which
   // every thread copies and reads its own slots (no barrier), kBeamRing steps
@@ -403,14 +407,12 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) beam_chunk_kernel(con
     }
   }
 
-  // this chunk's sum of 2^(x log2(e) - off), off = m log2(e) rounded: the join
-  // takes the same off, so its rounding cancels
-  const float off = m * kLog2e;
-  const bool huge = fabsf(m) >= kBeamHuge;  // x - m serves there
+  // This chunk's sum of exp(x - m). A logit far above all others counts as 1
+  // exactly, so that its log probability is 0.
   if (m == -INFINITY || best == -INFINITY) {
     my_sum = 0.0;
-  } else if (huge || !(my_sum < 1e30)) {
-    // rare (NaN, infinite or huge logits): from memory again, cleaned
+  } else if (!(my_sum < 1e30)) {
+    // rare (NaN or infinite logits): from memory again, cleaned
     my_sum = 0.0;
 #pragma unroll 1
     for (int i = 0; i < vectors; ++i) {
@@ -419,14 +421,11 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) beam_chunk_kernel(con
 #pragma unroll
       for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int e = 0; e < W::N; ++e) {
-          const float f = W::at(word[q], e);
-          my_sum += ex2(huge ? (f - m) * kLog2e : fmaf(f, kLog2e, -off));
-        }
+        for (int e = 0; e < W::N; ++e) my_sum += ex2((W::at(word[q], e) - m) * kLog2e);
     }
-  } else if (ref != -INFINITY) {
-    my_sum *= ex2(my_off - off);
-  }  // else: 0, nothing but masked logits
+  } else {
+    my_sum *= ex2((ref - m) * kLog2e);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) my_sum += __shfl_xor_sync(0xffffffffu, my_sum, o);
   if (lane == 0) s_sum[wid] = my_sum;
@@ -470,7 +469,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) beam_chunk_kernel(con
     double total = 0.0;
 #pragma unroll
     for (int k = 0; k < kBeamWarps; ++k) total += s_sum[k];
-    p.part_off[part] = huge ? m * 1.4426950408889634 : off;
+    p.part_off[part] = m * 1.4426950408889634;
     p.part_sum[part] = total;
   }
   uint64_t* out = p.part_key + part * K;

@@ -231,6 +231,35 @@ template <int N>
 __device__ __forceinline__ void bulk_wait_read_but() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
+// Two fp32 values in a register pair, added and multiplied by one instruction.
+struct F32x2 {
+  uint64_t v;
+  __device__ __forceinline__ F32x2(float a, float b) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  }
+  __device__ __forceinline__ explicit F32x2(uint64_t bits) : v(bits) {}
+  __device__ __forceinline__ float lo() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return a;
+  }
+  __device__ __forceinline__ float hi() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return b;
+  }
+  __device__ __forceinline__ F32x2 operator+(const F32x2& o) const {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(v), "l"(o.v));
+    return F32x2(r);
+  }
+  __device__ __forceinline__ F32x2 operator*(const F32x2& o) const {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(v), "l"(o.v));
+    return F32x2(r);
+  }
+};
+
 // One thread's 16-byte copies global -> shared (both aligned), counted in
 // groups; a group's bytes are visible to the thread that waited for it.
 __device__ __forceinline__ void copy_async16(void* dst, const void* src) {

@@ -1,8 +1,8 @@
 """Beam selection against a plain 64-bit implementation, and a beam search
 over the paged cache against one that keeps every beam's keys.
 
-Choices are whole numbers and are equal. Scores: a summand 2^(x log2(e) - off)
-carries the rounding of its exponent (below 8 for the summands that matter:
+Choices are whole numbers and are equal. Scores: a summand exp(x - ref)
+carries the roundings of its exponent (below 8 for the summands that matter:
 2^-22 ln 2 relative), of log2(e) and of the exponential (2^-22 each), its
 thread's four fp32 additions (2^-24 each) and the exponential that joins the
 thread to the others (2^-22): together below 1.2e-6 of the sum, which is as much
@@ -146,6 +146,22 @@ def test_masked_logits(beam, dtype):
     logits[3, 1, 77] = math.inf
     logits[3, 2, 2990] = math.nan
     check(beam, logits, scores, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab", [136, 50000])
+def test_certain_tokens_score_their_beam_exactly(beam, dtype, vocab):
+    """A token of probability 1 adds 0, so beams of equal scores that are each
+    certain of one tie, whatever its logit."""
+    g = torch.Generator().manual_seed(31)
+    logits = torch.full((4, 16, vocab), -90.0)
+    where = torch.randint(0, vocab, (4, 16), generator=g)
+    logits.scatter_(2, where[..., None], 20 * torch.randn(4, 16, 1, generator=g).clamp(-2, 2))
+    scores = torch.full((4, 16), -10.737407684326172, device=DEV)
+    best, parents, tokens = beam.beam_search_select(logits.to(dtype).to(DEV), scores, 16)
+    assert (best == scores).all()
+    assert torch.equal(parents.cpu().view(-1), torch.arange(64, dtype=torch.int32))
+    assert torch.equal(tokens.cpu(), where.int())
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
