@@ -1094,6 +1094,7 @@ struct DecodeAppend {
 // Sliding-window plan handed to decode_run (nullptr: full contexts). The
 // table arguments of decode_run are then the plan's compacted table.
 struct DecodeWindow {
+  int4 key;
   const int4* window;
   const int32_t* table_indptr;
   const int32_t* table_indices;
@@ -1155,6 +1156,7 @@ int decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_k
   p.counter = reinterpret_cast<int32_t*>(ws + L.counter);
   p.part_lse = reinterpret_cast<float*>(ws + L.part_lse);
   p.part_o = reinterpret_cast<float*>(ws + L.part_o);
+  p.window_key = win != nullptr ? win->key : int4{0, 0, 0, 0};
   p.window = win != nullptr ? win->window : nullptr;
   p.table_indptr = win != nullptr ? win->table_indptr : nullptr;
   p.table_indices = win != nullptr ? win->table_indices : nullptr;
@@ -1303,12 +1305,13 @@ int window_decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
       decode_ws_bytes(sh, batch_size, cache->num_kv_heads, cache->head_dim));
   if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const DecodeWindow win{reinterpret_cast<const int4*>(ws + L.window), kv_indptr, kv_indices};
+  const DecodeWindow win{
+      window_plan_key(window_left, num_sink_tokens, L.capacity, num_kv_indices),
+      reinterpret_cast<const int4*>(ws + L.window), kv_indptr, kv_indices};
   return decode_run(q, q_stride_n, q_stride_h, cache,
                     reinterpret_cast<const int32_t*>(ws + L.indices),
                     reinterpret_cast<const int32_t*>(ws + L.indptr), kv_last_page_len, batch_size,
-                    num_qo_heads, sm_scale, ws + L.decode, workspace_bytes - L.decode, out, lse,
-                    stream, app, &win);
+                    num_qo_heads, sm_scale, ws, L.indptr, out, lse, stream, app, &win);
 }
 
 }  // namespace

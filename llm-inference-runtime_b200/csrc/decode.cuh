@@ -92,14 +92,16 @@ __host__ __device__ inline bool decode_geom(int hkv, int head_dim, DecodeGeom* g
 // (request, head block, page) stream into runs of Q pages for `num_groups`
 // groups, clears the merge counters. kv_indptr is anything indexable
 // (a pointer, or a view that reads an indptr this CTA has just written);
-// `bad` is an error the caller has found already.
+// `bad_table` is an error the caller has found already, `key` what the run
+// has to be for beside batch and heads.
 template <typename Indptr>
 __device__ void decode_plan_block(const Indptr kv_indptr,
                                   const int32_t* __restrict__ last_len, int batch, int hkv,
                                   int hq, int head_dim, int page_size, int64_t num_indices,
                                   int num_groups, int hb, int min_per_group,
                                   uint8_t* __restrict__ ws, int32_t magic = kDecodeMagic,
-                                  bool bad_table = false, int max_pieces = 8) {
+                                  bool bad_table = false, int max_pieces = 8,
+                                  int4 key = {0, 0, 0, 0}) {
   const DecodeWsLayout L = decode_ws_layout(num_groups, batch, hkv, head_dim, hb);
   DecodePlanHeader* hdr = reinterpret_cast<DecodePlanHeader*>(ws + L.hdr);
   int4* unit_start = reinterpret_cast<int4*>(ws + L.unit_start);
@@ -173,6 +175,7 @@ __device__ void decode_plan_block(const Indptr kv_indptr,
     hdr->page_size = page_size;
     hdr->num_empty = err ? 0 : s_empty;
     hdr->heads_per_unit = hb;
+    hdr->key = key;
     hdr->magic = magic;
     if (err) set_status(PA_ERR_DEVICE_CHECK);
   }
@@ -386,6 +389,15 @@ __global__ void __launch_bounds__(decode_cta_warps(D) * 32, 1)
       hdr->num_qo_heads != p.num_qo_heads || hdr->head_dim != D || hdr->heads_per_unit != HB) {
     if (gw == 0 && lane == 0) set_status(PA_ERR_NOT_PLANNED);
     return;
+  }
+  if constexpr (kWindow) {
+    // before anything of the compacted table is read: it is this window's
+    const int4 k = hdr->key;
+    if (k.x != p.window_key.x || k.y != p.window_key.y || k.z != p.window_key.z ||
+        k.w != p.window_key.w) {
+      if (gw == 0 && lane == 0) set_status(PA_ERR_NOT_PLANNED);
+      return;
+    }
   }
   if (hdr->status != PA_OK) return;
   const int Q = hdr->per_unit, total = hdr->total, hkv = p.num_kv_heads, G = p.group;

@@ -46,7 +46,7 @@ struct DecodePlanHeader {
   int32_t page_size;
   int32_t num_empty;       // requests with zero pages (their output is zero)
   int32_t heads_per_unit;  // kv heads a group covers (one warp each)
-  int32_t reserved[4];
+  int4 key;                // a window plan's window and table size (window.cuh), else 0
 };
 
 // Byte offsets inside the caller's workspace. The stream of work is every
@@ -113,6 +113,7 @@ struct DecodeParams {
   // above are then the plan's compacted table of visible pages, window[b]
   // says what is hidden inside it, and table_indptr / table_indices are the
   // caller's own table (an append may go to a page that is not visible).
+  int4 window_key;  // the plan's header has the same (window_plan_key)
   const int4* window;
   const int32_t* table_indptr;
   const int32_t* table_indices;

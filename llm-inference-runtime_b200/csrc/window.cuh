@@ -50,11 +50,22 @@ __host__ __device__ inline WindowSpan window_span(int64_t first_query, int windo
   return w;
 }
 
-// Workspace of a window decode: the compacted table, then the decode plan.
+// Workspace of a window decode: the decode plan, whose header is at offset 0 as
+// every plan's is, then the compacted table. A plan of any other kind over the
+// same workspace so replaces the header, whatever else it leaves standing.
 struct WindowDecodeWsLayout {
-  size_t indptr, window, indices, decode, total;
+  size_t indptr, window, indices, total;
   int64_t capacity;  // page ids the compacted table holds
 };
+
+// What the header says of a window plan beside the batch and the heads: a run
+// for another window or another table's size is refused.
+__host__ __device__ inline int4 window_plan_key(int window, int sinks, int64_t capacity,
+                                                int64_t num_indices) {
+  constexpr int64_t kMost = 0x7fffffff;
+  return make_int4(window, sinks, static_cast<int>(capacity < kMost ? capacity : kMost),
+                   static_cast<int>(num_indices < kMost ? num_indices : kMost));
+}
 
 // Pages of one request's stream at most: the sinks', and the window's
 // window + 1 keys over one page more than they fill.
@@ -68,15 +79,14 @@ __host__ __device__ inline WindowDecodeWsLayout window_decode_ws_layout(
   WindowDecodeWsLayout L;
   const int64_t most = window_pages_max(window, sinks, page_size) * batch;
   L.capacity = most < num_indices ? most : num_indices;
-  size_t o = 0;
+  size_t o = decode_bytes;
   L.indptr = o;
   o = align256(o + 4 * (static_cast<size_t>(batch) + 1));
   L.window = o;  // int4 {hole_lo, hole_hi, sink_pages, shift} per request
   o = align256(o + sizeof(int4) * static_cast<size_t>(batch));
   L.indices = o;
   o = align256(o + 4 * static_cast<size_t>(L.capacity));
-  L.decode = o;
-  L.total = o + decode_bytes;
+  L.total = o;
   return L;
 }
 
@@ -186,8 +196,8 @@ __global__ void __launch_bounds__(kWindowPlanThreads)
       __syncthreads();
     }
     decode_plan_block(FreshIndptr{s_held, out_indptr}, last_len, batch, hkv, hq, head_dim, page_size,
-                      L.capacity, num_groups, hb, min_per_group, ws + L.decode,
-                      kWindowDecodeMagic, s_bad != 0, max_pieces);
+                      L.capacity, num_groups, hb, min_per_group, ws, kWindowDecodeMagic, s_bad != 0,
+                      max_pieces, window_plan_key(window, sinks, L.capacity, num_indices));
     return;
   }
   int32_t* out_indices = reinterpret_cast<int32_t*>(ws + L.indices);
