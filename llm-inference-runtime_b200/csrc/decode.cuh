@@ -319,12 +319,15 @@ __device__ __noinline__ void merge_segments(const float* part_lse, const float* 
 }
 
 // Row b's new token of head `head` written into the pool alone: slot `slot`
-// of page `rp` of the caller's table (one 16-byte chunk per lane).
+// of page `rp` of the caller's table (one 16-byte chunk per lane). The table
+// may be another one than was planned, so its row is measured here.
 template <int D>
 __device__ __forceinline__ void append_row_to_pool(const DecodeParams& p, int b, int head, int rp,
                                                 int slot, int lane) {
   constexpr int CH = D / 8;
-  const int page = __ldg(p.table_indices + __ldg(p.table_indptr + b) + rp);
+  const int first = __ldg(p.table_indptr + b), end = __ldg(p.table_indptr + b + 1);
+  const bool inside = first >= 0 && end <= p.window_key.w && rp < end - first;
+  const int page = inside ? __ldg(p.table_indices + first + rp) : -1;
   if (page < 0 || page >= p.num_pages) {
     if (lane == 0) set_status(PA_ERR_DEVICE_CHECK);
     return;

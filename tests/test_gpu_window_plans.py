@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_window import DEV, HUGE, P, Problem, _decode_problem, _decode_wrapper, _t, _ws
+from test_gpu_window import DEV, HUGE, P, _decode_problem, _decode_wrapper, _t, _ws
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +121,25 @@ def test_refused_runs_in_a_graph_report_the_plan(fi, lir):
             assert (out == 7).all()
     finally:
         fi._CHECK = saved
+
+
+def test_an_append_stays_inside_the_rows_of_the_callers_table(fi):
+    """Two tables of one size whose rows have other lengths, one workspace: a
+    run of the first on the plan of the second takes a position that only the
+    planned row has. It is reported and not written to the next row's pages."""
+    a = _decode_problem([40, 400], 8, 2, 64, 40, 4, seed=11, poison=False, evict=False)
+    b = _decode_problem([400, 40], 8, 2, 64, 40, 4, seed=11, poison=False, evict=False)
+    ws, q, pool = _ws(), a.q.to(DEV), a.device_pool()
+    w = _decode_wrapper(fi, a, ws)
+    _decode_wrapper(fi, b, ws)
+    before = pool.clone()
+    k = torch.ones((2, 2, 64), dtype=a.dtype, device=DEV)
+    with pytest.raises(RuntimeError, match="device"):
+        w.run_with_append(q, pool, k, k, _t([100, 2]))  # page 6 of a row of three
+    beyond = a.tables[1][6 - 3]
+    assert torch.equal(pool[beyond].view(torch.int16), before[beyond].view(torch.int16))
+    # on its own plan the position is refused by the row's length
+    w.plan(_t(a.indptr), _t(a.indices), _t(a.last), 8, 2, 64, P, q_data_type=a.dtype)
+    with pytest.raises(RuntimeError, match="device"):
+        w.run_with_append(q, pool, k, k, _t([100, 2]))
+    assert torch.equal(pool[beyond].view(torch.int16), before[beyond].view(torch.int16))
