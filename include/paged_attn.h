@@ -204,7 +204,10 @@ int pa_fork_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
  *     page of tokens [j * page_size, (j + 1) * page_size) of a row, -1 = given back
  *   seq_lens[rows]          tokens a row holds; its entries j < ceil(len / page_size).
  *     Between pa_fork_sequences and the append of the row's token, lengths that
- *     count this token (len + 1) hold its page too.
+ *     count this token (len + 1, but no more than max_blocks * page_size: a row
+ *     whose table is full has no place for it) hold its page too. A length past
+ *     the table is an error; pa_release_pages leaves that row as it is,
+ *     pa_compact_pages has its max_blocks entries follow the pages.
  * Errors that only the device sees (a page id outside the pool, a count that
  * falls below zero, no free page left) are recorded as PA_ERR_DEVICE_CHECK and
  * counted in counts[2] where its line says so; sound rows are processed all
@@ -247,7 +250,8 @@ int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers
  * the k-th live page at or past n goes to the k-th free page before n, in all
  * layers. ref_counts follow, the tables' entries too; remap[num_pages]
  * receives each live page's new number, -1 for free ones (for holders outside
- * the tables). counts receives {live pages, pages moved, errors}. workspace:
+ * the tables). counts receives {live pages, pages moved, errors: entries whose
+ * page nobody holds (they stay), rows whose length is not one}. workspace:
  * num_pages + 2 int32. */
 int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
                      int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,

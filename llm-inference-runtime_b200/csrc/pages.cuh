@@ -582,15 +582,18 @@ __global__ void __launch_bounds__(kReleaseThreads) remap_tables_kernel(const Rem
   const int b = blockIdx.x;
   const int len = __ldg(p.lens + b);
   int32_t* row = p.tables + b * p.stride;
-  const bool bad = len < 0 || len > static_cast<int64_t>(p.width) * p.page_size;
-  const int n = bad ? 0 : static_cast<int>((static_cast<int64_t>(len) + p.page_size - 1) / p.page_size);
-  int errors = bad && threadIdx.x == 0 ? 1 : 0;
+  // A length past the table is reported once, and the entries that there are
+  // follow all the same: their pages have moved.
+  const bool past = len > static_cast<int64_t>(p.width) * p.page_size;
+  const int64_t held = (static_cast<int64_t>(len) + p.page_size - 1) / p.page_size;
+  const int n = len < 0 ? 0 : past ? p.width : static_cast<int>(held);
+  int errors = (len < 0 || past) && threadIdx.x == 0 ? 1 : 0;
   for (int j = threadIdx.x; j < n; j += kReleaseThreads) {
     const int page = row[j];
     if (page < 0) continue;
     const int to = page < p.num_pages ? __ldcg(p.remap + page) : -1;
     if (to < 0) {
-      ++errors;  // a page that nobody holds: the entry stays
+      errors += !past;  // a page that nobody holds: the entry stays
       continue;
     }
     if (to != page) row[j] = to;

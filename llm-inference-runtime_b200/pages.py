@@ -11,8 +11,11 @@ step that reorders beams or gives pages back can be captured in a CUDA graph:
 * ``seq_lens`` [sequences]: tokens a sequence holds; its pages are the first
   ceil(seq_len / 16) entries, and what lies behind them is not read. Between a
   fork and the append of its token the page of that token is held too: a call
-  there counts it (``free_sequences(tables, seq_lens + 1, refs)``,
-  ``compact_pages(pool, tables, seq_lens + 1, refs)``).
+  there counts it, as far as the table has room (``held = (seq_lens + 1).clamp(
+  max=16 * max_blocks)``, then ``free_sequences(tables, held, refs)`` or
+  ``compact_pages(pool, tables, held, refs)``). A length past the table is an
+  error: ``free_sequences`` and ``evict_window_pages`` leave such a row as it
+  is, ``compact_pages`` updates the entries that there are.
 
 Each call returns ``counts``, an int32 device tensor of three; its last entry
 counts what could not be done (it stays 0 in a sound step), which is also
@@ -191,7 +194,7 @@ def compact_pages(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: t
     follow. Returns (remap, counts): remap [pages] is each live page's new
     number, -1 for free ones, for holders outside the tables (a prefix
     cache); counts: live pages, pages moved, errors (entries whose page
-    nobody holds; they stay)."""
+    nobody holds, which stay, and rows whose length is past the table)."""
     device = _state(block_tables, seq_lens, ref_counts)
     ptr, layer_stride, layers, page_stride, page_bytes, pages = _pool(kv_pool, ref_counts)
     remap, counts = ref_counts.new_empty(pages), ref_counts.new_empty(3)
