@@ -232,8 +232,12 @@ int pa_release_pages(int32_t* block_tables, int64_t block_table_stride, int32_t 
  * of page_size; otherwise the parent's unfinished page, which its first
  * continuing row keeps if no other holder is left, while every other one gets
  * a free page and a copy of it in all layers. Rows nobody continues lose
- * their references. Free pages (count 0 once all references are counted) are
- * taken lowest number first, by ascending r. Entries past the row's are -1.
+ * their references. A row whose parent is -1 has ended: its length is 0, its
+ * entries are -1, it takes no page. (A row of length 0 that continues takes the
+ * page of its first token; forked again without that token it takes another,
+ * and nothing gives the first one back.) Free pages (count 0 once all
+ * references are counted) are taken lowest number first, by ascending r.
+ * Entries past the row's are -1.
  * counts receives {pages copied, pages taken, rows left without a page (their
  * entry is -1)}. pool, strides and page_bytes as for pa_fork_pages;
  * out_block_tables must not overlap block_tables; workspace: 3 * num_sequences

@@ -10,7 +10,7 @@ continuations of each request's beams, and the cache following them
 from __future__ import annotations
 
 import functools
-from typing import Dict, Tuple
+from typing import Dict, Optional, Tuple
 
 import torch
 
@@ -83,8 +83,8 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
 
 def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.Tensor,
                      block_tables: torch.Tensor, seq_lens: torch.Tensor,
-                     ref_counts: torch.Tensor, kv_layout: str = "HND"
-                     ) -> Dict[str, torch.Tensor]:
+                     ref_counts: torch.Tensor, kv_layout: str = "HND",
+                     active: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
     """One step of beam search: each request's beams are replaced by its
     ``beams`` best continuations and their cache follows.
 
@@ -93,11 +93,24 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.
     block_tables, seq_lens and counts (``pages.fork_sequences``): every beam
     owns the page that its token, to be fed to the model next, is appended
     to, at position seq_lens[r] (the lengths to pass to the next step are these
-    plus one)."""
+    plus one).
+
+    ``active`` [batch] bool: requests that go on. The rows of the others end,
+    in this step and in every later one that names them: they give up their
+    pages, take none, and come back with parent -1, length 0 (which stays 0)
+    and a table of -1. Their scores and tokens mean nothing. Without it every
+    row takes the page of its next token, a row without a continuation (score
+    -inf) or of length 0 too, so a request that has ended has to be named:
+    ``active=(scores > -inf).any(1)``, where its scores say so."""
     batch, beams = scores.shape
     if seq_lens.numel() != batch * beams:
         raise ValueError("block_tables must hold one row per beam of each request")
+    if active is not None and (active.dtype != torch.bool or active.shape != (batch,)
+                               or active.device != logits.device):
+        raise ValueError("active must be a bool tensor of one entry per request, on the same GPU")
     best, parents, tokens = beam_search_select(logits, scores, beams)
+    if active is not None:
+        parents = parents.masked_fill(~active[:, None], -1)
     tables, lens, counts = pages.fork_sequences(kv_pool, block_tables, seq_lens,
                                                 parents.view(-1), ref_counts,
                                                 kv_layout=kv_layout)

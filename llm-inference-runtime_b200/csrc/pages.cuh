@@ -274,6 +274,9 @@ __device__ __forceinline__ void load_counts(const int32_t* refs, int64_t at, int
 //     - else the parent's unfinished page: its holders among the old rows let
 //       go of it; if nobody else holds it the first row that continues it
 //       keeps it, every other one gets a free page and a copy.
+// A row with parent -1 ends: it holds nothing. (A row of length 0 that goes on
+// takes a page like any other, which it would hold until its next token; a row
+// that stays in the batch without going on has to say so.)
 // Three launches: per row (counts of the full pages, the gathered table),
 // one CTA (who keeps, who gets which page), the copies.
 struct ForkSeqParams {
@@ -297,11 +300,13 @@ struct ForkSeqParams {
 struct ForkRow {
   int parent, len, full, last;  // last: the unfinished page, -1: none (or given back)
   bool ok;                      // parent and length are sound
+  bool ended;                   // continues nothing, and is not meant to
 };
 
 __device__ __forceinline__ ForkRow fork_row(const ForkSeqParams& p, int r) {
   ForkRow f;
   f.parent = __ldg(p.parents + r);
+  f.ended = f.parent == -1;
   f.ok = f.parent >= 0 && f.parent < p.rows;
   f.len = f.ok ? __ldg(p.lens + f.parent) : 0;
   if (f.len < 0 || f.len > static_cast<int64_t>(p.width) * p.page_size) f.ok = false;
@@ -370,7 +375,7 @@ __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeq
   __shared__ int s_avail[kScanThreads];
   const int tid = threadIdx.x;
   const int rounds = (p.rows + kScanThreads - 1) / kScanThreads;
-  const ForkRow none{0, 0, 0, -1, false};
+  const ForkRow none{0, 0, 0, -1, false, true};
   const ForkRow first = tid < p.rows ? fork_row(p, tid) : none;
   int state0 = 0;  // state of row `tid`; later rows' in p.state
   auto row = [&](int k) {
@@ -413,7 +418,7 @@ __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeq
       p.out_tables[r * p.out_stride + f.full] = f.last;
     }
     // state: rank among the rows that want a page, -1: wants none (keeps its
-    // page, or is not sound)
+    // page, has ended, or is not sound)
     const bool wants = r < p.rows && f.ok && !keep && f.full < p.width;
     int n;
     const int at = total + block_exclusive(wants ? 1 : 0, s_warp, &n);
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeq
         missing += page < 0;
       } else if (!f.ok || f.full >= p.width) {
         if (f.full < p.width) p.out_tables[r * p.out_stride + f.full] = -1;
-        ++missing;
+        missing += !f.ended;
       }
     }
     int n;

@@ -149,13 +149,16 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
     size, otherwise the parent's unfinished page, kept by the first sequence
     that continues it if nobody else holds it and copied (all layers) into a
     free page for the others. Sequences that nobody continues give up their
-    pages. Free pages are those with count 0, taken lowest number first.
+    pages; ``parents[r] = -1`` ends sequence r (length 0, entries -1, no page).
+    Free pages are those with count 0, taken lowest number first.
     counts: pages copied, pages taken, sequences left without a page (their
     entry is -1: the pool is full, or the table has no room).
 
     A sequence's token is appended (at position seq_lens[r], which then grows
-    by one) before it is forked again. ``out`` receives the new tables, for
-    example the other half of a double buffer."""
+    by one) before it is forked again: a page taken for a token that never came
+    is not found again by the next fork. A sequence that stays in the batch
+    without going on, of length 0 too, has parent -1 for that reason. ``out``
+    receives the new tables, for example the other half of a double buffer."""
     device = _state(block_tables, seq_lens, ref_counts)
     _on_gpu_i32(parents, "parents", 1)
     if parents.numel() != seq_lens.numel() or parents.device != device:

@@ -82,3 +82,143 @@ def test_release_leaves_a_row_past_its_table(pages, fi, lir):
         assert t[0].tolist() == [0, 1] and n[0] == 2 * P + 1 and c[:2].tolist() == [1, 1]
     want_t, want_r, _ = plain_release(tables[1:], np.array([2 * P]), refs, 0, 0)
     assert t[1].tolist() == want_t[0].tolist() and c.tolist() == want_r.tolist()
+
+
+# ---------------------------------------------------------- sequences that have ended
+def plain_fork(tables, lens, refs, parents):
+    """(tables, lens, refs, counts, copies), with -1 for a parent of none."""
+    rows, width = tables.shape
+    refs, out, out_lens = refs.copy(), np.full_like(tables, -1), np.zeros_like(lens)
+    for r in range(rows):
+        for page in tables[r, :-(-lens[r] // P)]:
+            if page >= 0:
+                refs[page] -= 1
+    alive = [r for r in range(rows) if parents[r] != -1]
+    for r in alive:
+        s = parents[r]
+        out_lens[r] = lens[s]
+        for j in range(lens[s] // P):
+            out[r, j] = tables[s, j]
+            if out[r, j] >= 0:
+                refs[out[r, j]] += 1
+    last = {r: int(tables[parents[r], out_lens[r] // P]) for r in alive if out_lens[r] % P}
+    held = {page for page in last.values() if refs[page] > 0}
+    kept, wants, missing = set(), [], 0
+    for r in alive:
+        at = out_lens[r] // P
+        if r in last and last[r] not in held | kept:
+            kept.add(last[r])
+            refs[last[r]] += 1
+            out[r, at] = last[r]
+        elif at < width:
+            wants.append(r)
+        else:
+            missing += 1
+    free = [i for i in range(len(refs)) if refs[i] == 0]
+    copies = []
+    for r, page in zip(wants, free):
+        out[r, out_lens[r] // P] = page
+        refs[page] = 1
+        if r in last:
+            copies.append((last[r], page))
+    missing += max(len(wants) - len(free), 0)
+    return out, out_lens, refs, [len(copies), min(len(wants), len(free)), missing], copies
+
+
+def _fork(pages, pool, t, n, parents, c):
+    """One fork against the plain one; returns the new state."""
+    tables, lens, refs = (x.cpu().numpy().astype(np.int64) for x in (t, n, c))
+    want_t, want_l, want_r, want_c, copies = plain_fork(tables, lens, refs, parents)
+    want_pool = _copied(pool, copies)
+    t, n, counts = pages.fork_sequences(pool, t, n, _i32(parents), c)
+    assert counts.tolist() == want_c
+    assert np.array_equal(t.cpu().numpy(), want_t) and np.array_equal(n.cpu().numpy(), want_l)
+    assert np.array_equal(c.cpu().numpy(), want_r)
+    assert torch.equal(_bits(pool), _bits(want_pool))
+    return t, n
+
+
+def _references(tables, total):
+    live = tables[tables >= 0].long()
+    return torch.zeros(total, dtype=torch.int32, device=DEV).index_add_(
+        0, live, torch.ones_like(live, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("rows", [1, 5, 40, 1300])
+def test_fork_of_rows_that_end(pages, seed, rows):
+    """Any rows end, with and without rows that continue them, and stay ended."""
+    rng = np.random.RandomState(100 * seed + rows)
+    lens = rng.randint(0, 70, rows)
+    total = 10 * rows
+    tables = np.full((rows, 6), -1, dtype=np.int64)
+    ids = rng.permutation(total).tolist()
+    for r in range(rows):
+        for j in range(-(-lens[r] // P)):
+            tables[r, j] = ids.pop()
+    t, n, pool = _i32(tables), _i32(lens), _pool(total, 1, 1, 8)
+    c = _references(t, total)
+    for step in range(3):
+        parents = rng.randint(0, rows, rows)
+        parents[rng.rand(rows) < (1.0 if seed == 0 and step == 1 else 0.4)] = -1
+        t, n = _fork(pages, pool, t, n, parents, c)
+        # (the token to come of the rows that go on is appended)
+        n += _i32(parents >= 0)
+        assert torch.equal(c, _references(t, total))
+    pages.free_sequences(t, n, c)
+    assert (c == 0).all()
+
+
+@pytest.mark.parametrize("how", ["freed", "stopped", "ended with its pages"])
+def test_beam_search_steps_beside_a_request_that_has_ended(pages, fi, how):
+    """Of three requests the second ends; in every later step the counts are
+    the tables' own, and the pool does not drain."""
+    beam = importlib.import_module("llm-inference-runtime_b200.beam")
+    batch, beams, vocab, total, prompt = 3, 4, 60, 64, 2 * P
+    rows = batch * beams
+    g = torch.Generator().manual_seed(7)
+    pool = _pool(total, 2, 1, 8)
+    t = torch.full((rows, 8), -1, dtype=torch.int32, device=DEV)
+    t[:, :2] = torch.arange(rows * 2, device=DEV).view(rows, 2).int()
+    n = torch.full((rows,), prompt, dtype=torch.int32, device=DEV)
+    c = _references(t, total)
+    scores = -torch.rand(batch, beams, generator=g).to(DEV)
+    active = torch.ones(batch, dtype=torch.bool, device=DEV)
+    most = 0
+    for step in range(40):
+        if step == 5:
+            mine = slice(beams, 2 * beams)
+            if how == "freed":  # (the step's tokens are in: lengths are what the rows hold)
+                pages.free_sequences(t[mine], n[mine], c)
+            elif how == "stopped":
+                scores[1] = -float("inf")
+            active[1] = False
+        if how == "stopped":
+            active = (scores > -float("inf")).any(1)
+        logits = (torch.randn(batch, beams, vocab, generator=g) * 2).to(DEV)
+        got = beam.beam_search_step(logits, scores, pool, t, n, c, active=active)
+        assert got["counts"][2] == 0
+        t, n, scores = got["block_tables"], got["seq_lens"], got["scores"]
+        on = active.repeat_interleave(beams)
+        if step >= 5:
+            assert (got["parents"][1] == -1).all() and (t[~on] == -1).all() and (n[~on] == 0).all()
+            if how == "stopped":
+                scores[1] = -float("inf")
+        assert torch.equal(got["parents"].view(-1)[on] // beams,
+                           torch.arange(batch, device=DEV).int().repeat_interleave(beams)[on])
+        n = n + on
+        assert (n[on] == prompt + step + 1).all() and (t[on, (prompt + step) // P] >= 0).all()
+        assert torch.equal(c, _references(t, total))
+        most = max(most, int((c > 0).sum()))
+    assert most < total
+    assert int((c > 0).sum()) <= 2 * beams * 5
+
+
+def test_active_is_checked(fi):
+    beam = importlib.import_module("llm-inference-runtime_b200.beam")
+    x, s = torch.zeros(2, 3, 10, device=DEV), torch.zeros(2, 3, device=DEV)
+    n, t, c = _i32(np.zeros(6)), _i32(np.zeros((6, 2))), _i32(np.ones(4))
+    for bad in (torch.ones(2, device=DEV), torch.ones(3, dtype=torch.bool, device=DEV),
+                torch.ones(2, 3, dtype=torch.bool, device=DEV), torch.ones(2, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="active"):
+            beam.beam_search_step(x, s, _pool(4), t, n, c, active=bad)
