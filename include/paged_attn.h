@@ -73,10 +73,10 @@ const char* pa_status_string(int status);
 /* ABI version this header describes (major * 100 + minor). 101: the append,
  * RoPE + append, fused QKV and cascade-plan calls take the number of page ids
  * (num_kv_indices) after kv_indptr. 102: the pa_window_* calls,
- * pa_release_pages, pa_fork_sequences, pa_compact_pages, pa_beam_select. A
- * caller built against another version must refuse the library (the Python
- * binding does). */
-#define PA_ABI_VERSION 102
+ * pa_release_pages, pa_fork_sequences, pa_compact_pages, pa_beam_select. 103:
+ * pa_fork_held_sequences. A caller built against another version must refuse
+ * the library (the Python binding does). */
+#define PA_ABI_VERSION 103
 
 /* ABI version of this library (major * 100 + minor); equals PA_ABI_VERSION
  * of the header it was built from. */
@@ -241,7 +241,11 @@ int pa_release_pages(int32_t* block_tables, int64_t block_table_stride, int32_t 
  * counts receives {pages copied, pages taken, rows left without a page (their
  * entry is -1)}. pool, strides and page_bytes as for pa_fork_pages;
  * out_block_tables must not overlap block_tables; workspace: 3 * num_sequences
- * int32. */
+ * int32. A parent's unfinished page that its table does not name (-1) counts as
+ * given back: its rows go on in free pages, whose first len % page_size tokens
+ * are not theirs (a caller that gives such pages back hides them). That is also
+ * what this call leaves of a row whose unfinished page it could not copy, so
+ * after counts[2] it is pa_fork_held_sequences that tells the two apart. */
 int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
                       int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
                       const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
@@ -249,6 +253,19 @@ int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers
                       int32_t page_size, int32_t* ref_counts, int32_t* out_block_tables,
                       int64_t out_stride, int32_t* out_seq_lens, int32_t* counts,
                       int32_t* workspace, void* stream);
+
+/* pa_fork_sequences for callers that never give back an unfinished page
+ * (pa_release_pages does not): one that the table does not name is lost, with
+ * its tokens. Rows that continue it count in counts[2], take no page and come
+ * back with the length of their full pages, and so does a row that finds no
+ * free page for its copy: what the new lengths count is in the pages. */
+int pa_fork_held_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                           int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                           const int32_t* block_tables, int64_t block_table_stride,
+                           int32_t max_blocks, const int32_t* seq_lens, const int32_t* parents,
+                           int32_t num_sequences, int32_t page_size, int32_t* ref_counts,
+                           int32_t* out_block_tables, int64_t out_stride, int32_t* out_seq_lens,
+                           int32_t* counts, int32_t* workspace, void* stream);
 
 /* Moves the live pages (count > 0) to the front of the pool: with n of them,
  * the k-th live page at or past n goes to the k-th free page before n, in all

@@ -34,7 +34,7 @@ PA_NOALLOC_SCRATCH_BYTES = 24 * 1024 * 1024
 
 # PA_ABI_VERSION of include/paged_attn.h that SIGNATURES mirrors; a library
 # reporting another version is refused (argument lists would not line up).
-ABI_VERSION = 102
+ABI_VERSION = 103
 
 
 class PagedKVCache(ctypes.Structure):
@@ -101,6 +101,12 @@ SIGNATURES = {
          c_int64, c_void_p, c_void_p],
     ),
     "pa_fork_sequences": (
+        c_int32,
+        [c_void_p, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
+         c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+         c_void_p, c_void_p],
+    ),
+    "pa_fork_held_sequences": (
         c_int32,
         [c_void_p, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
          c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,

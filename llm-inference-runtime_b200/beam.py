@@ -93,7 +93,9 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.
     block_tables, seq_lens and counts (``pages.fork_sequences``): every beam
     owns the page that its token, to be fed to the model next, is appended
     to, at position seq_lens[r] (the lengths to pass to the next step are these
-    plus one).
+    plus one). A beam for which the pool had no page is counted in counts[2] and
+    keeps its full pages only (``all_held`` there): until it is ended, each step
+    counts it again.
 
     ``active`` [batch] bool: requests that go on. The rows of the others end,
     in this step and in every later one that names them: they give up their
@@ -113,6 +115,6 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.
         parents = parents.masked_fill(~active[:, None], -1)
     tables, lens, counts = pages.fork_sequences(kv_pool, block_tables, seq_lens,
                                                 parents.view(-1), ref_counts,
-                                                kv_layout=kv_layout)
+                                                kv_layout=kv_layout, all_held=True)
     return {"scores": best, "parents": parents, "tokens": tokens, "block_tables": tables,
             "seq_lens": lens, "counts": counts}

@@ -678,13 +678,17 @@ int pa_release_pages(int32_t* block_tables, int64_t block_table_stride, int32_t 
   return launch_chain(release_pages_kernel, dim3(batch_size), dim3(kReleaseThreads), 0, s, p);
 }
 
-int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
-                      int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
-                      const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
-                      const int32_t* seq_lens, const int32_t* parents, int32_t num_sequences,
-                      int32_t page_size, int32_t* ref_counts, int32_t* out_block_tables,
-                      int64_t out_stride, int32_t* out_seq_lens, int32_t* counts,
-                      int32_t* workspace, void* stream) {
+}  // extern "C"
+
+namespace {
+
+int fork_sequences(bool all_held, void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                   int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                   const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                   const int32_t* seq_lens, const int32_t* parents, int32_t num_sequences,
+                   int32_t page_size, int32_t* ref_counts, int32_t* out_block_tables,
+                   int64_t out_stride, int32_t* out_seq_lens, int32_t* counts, int32_t* workspace,
+                   void* stream) {
   int st = check_pool(pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
                       num_pages);
   if (st != PA_OK) return st;
@@ -713,6 +717,7 @@ int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers
   p.out_stride = out_stride;
   p.out_lens = out_seq_lens;
   p.counts = counts;
+  p.all_held = all_held;
   p.avail = workspace;
   p.dst = workspace + num_sequences;
   p.state = workspace + 2 * static_cast<int64_t>(num_sequences);
@@ -722,6 +727,36 @@ int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers
   if (st != PA_OK || num_layers == 0 || page_bytes == 0) return st;
   return launch_copy_pages(pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
                            p.state, p.dst, counts, num_sequences, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pa_fork_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                      int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                      const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks,
+                      const int32_t* seq_lens, const int32_t* parents, int32_t num_sequences,
+                      int32_t page_size, int32_t* ref_counts, int32_t* out_block_tables,
+                      int64_t out_stride, int32_t* out_seq_lens, int32_t* counts,
+                      int32_t* workspace, void* stream) {
+  return fork_sequences(false, pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
+                        num_pages, block_tables, block_table_stride, max_blocks, seq_lens, parents,
+                        num_sequences, page_size, ref_counts, out_block_tables, out_stride,
+                        out_seq_lens, counts, workspace, stream);
+}
+
+int pa_fork_held_sequences(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
+                           int64_t page_stride_bytes, int64_t page_bytes, int64_t num_pages,
+                           const int32_t* block_tables, int64_t block_table_stride,
+                           int32_t max_blocks, const int32_t* seq_lens, const int32_t* parents,
+                           int32_t num_sequences, int32_t page_size, int32_t* ref_counts,
+                           int32_t* out_block_tables, int64_t out_stride, int32_t* out_seq_lens,
+                           int32_t* counts, int32_t* workspace, void* stream) {
+  return fork_sequences(true, pool, layer_stride_bytes, num_layers, page_stride_bytes, page_bytes,
+                        num_pages, block_tables, block_table_stride, max_blocks, seq_lens, parents,
+                        num_sequences, page_size, ref_counts, out_block_tables, out_stride,
+                        out_seq_lens, counts, workspace, stream);
 }
 
 int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,

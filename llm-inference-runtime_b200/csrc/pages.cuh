@@ -277,6 +277,12 @@ __device__ __forceinline__ void load_counts(const int32_t* refs, int64_t at, int
 // A row with parent -1 ends: it holds nothing. (A row of length 0 that goes on
 // takes a page like any other, which it would hold until its next token; a row
 // that stays in the batch without going on has to say so.)
+// An unfinished page that the table does not name (-1): with all_held it is
+// lost (an earlier fork found no free page for the row), and so are its tokens.
+// The row is reported, takes no page (a free one holds some other sequence's
+// tokens) and comes back with the length of its full pages, as does a row that
+// this fork leaves without the copy. Without all_held it counts as given back
+// behind a window, and the row goes on in a free page.
 // Three launches: per row (counts of the full pages, the gathered table),
 // one CTA (who keeps, who gets which page), the copies.
 struct ForkSeqParams {
@@ -291,6 +297,7 @@ struct ForkSeqParams {
   int64_t out_stride;
   int32_t* out_lens;
   int32_t* counts;  // copies, pages taken, rows left without a page
+  bool all_held;    // no unfinished page was given back
   // scratch, [rows] each
   int32_t* avail;  // free pages, lowest number first
   int32_t* dst;    // copies: to
@@ -301,6 +308,7 @@ struct ForkRow {
   int parent, len, full, last;  // last: the unfinished page, -1: none (or given back)
   bool ok;                      // parent and length are sound
   bool ended;                   // continues nothing, and is not meant to
+  bool lost;                    // its unfinished page is not there
 };
 
 __device__ __forceinline__ ForkRow fork_row(const ForkSeqParams& p, int r) {
@@ -313,10 +321,15 @@ __device__ __forceinline__ ForkRow fork_row(const ForkSeqParams& p, int r) {
   if (!f.ok) f.len = 0;
   f.full = f.len / p.page_size;
   f.last = -1;
+  f.lost = false;
   if (f.len % p.page_size) {
     f.last = __ldg(p.tables + f.parent * p.stride + f.full);
     if (f.last >= p.num_pages) f.ok = false;
-    if (f.last < 0) f.last = -1;  // given back: nothing to keep or copy
+    if (f.last < 0) {  // nothing to keep or copy
+      f.last = -1;
+      f.lost = p.all_held;
+      if (f.lost) f.len = f.full * p.page_size;
+    }
   }
   return f;
 }
@@ -375,7 +388,7 @@ __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeq
   __shared__ int s_avail[kScanThreads];
   const int tid = threadIdx.x;
   const int rounds = (p.rows + kScanThreads - 1) / kScanThreads;
-  const ForkRow none{0, 0, 0, -1, false, true};
+  const ForkRow none{0, 0, 0, -1, false, true, false};
   const ForkRow first = tid < p.rows ? fork_row(p, tid) : none;
   int state0 = 0;  // state of row `tid`; later rows' in p.state
   auto row = [&](int k) {
@@ -418,8 +431,8 @@ __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeq
       p.out_tables[r * p.out_stride + f.full] = f.last;
     }
     // state: rank among the rows that want a page, -1: wants none (keeps its
-    // page, has ended, or is not sound)
-    const bool wants = r < p.rows && f.ok && !keep && f.full < p.width;
+    // page, has lost it, has ended, or is not sound)
+    const bool wants = r < p.rows && f.ok && !f.lost && !keep && f.full < p.width;
     int n;
     const int at = total + block_exclusive(wants ? 1 : 0, s_warp, &n);
     total += n;
@@ -468,7 +481,8 @@ __global__ void __launch_bounds__(kScanThreads) fork_assign_kernel(const ForkSeq
         }
         p.out_tables[r * p.out_stride + f.full] = page;
         missing += page < 0;
-      } else if (!f.ok || f.full >= p.width) {
+        if (page < 0 && p.all_held) p.out_lens[r] = f.full * p.page_size;
+      } else if (!f.ok || f.lost || f.full >= p.width) {
         if (f.full < p.width) p.out_tables[r * p.out_stride + f.full] = -1;
         missing += !f.ended;
       }

@@ -137,8 +137,8 @@ def free_sequences(block_tables: torch.Tensor, seq_lens: torch.Tensor, ref_count
 
 def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                    parents: torch.Tensor, ref_counts: torch.Tensor,
-                   out: Optional[torch.Tensor] = None, kv_layout: str = "HND"
-                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                   out: Optional[torch.Tensor] = None, kv_layout: str = "HND",
+                   all_held: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Sequence r continues sequence ``parents[r]``: beam search's reordering
     of states, or several samples of one prompt. Returns (block_tables,
     seq_lens, counts) of the new sequences; ``ref_counts`` and ``kv_pool`` are
@@ -153,6 +153,15 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
     Free pages are those with count 0, taken lowest number first.
     counts: pages copied, pages taken, sequences left without a page (their
     entry is -1: the pool is full, or the table has no room).
+
+    A sequence whose unfinished page could not be copied has lost that page's
+    tokens. ``all_held=True`` says that no unfinished page was given back (no
+    call here does that), so that one missing from a table is known to be lost:
+    such a sequence comes back with the length of its full pages, without a
+    page, counted as above, in this fork and in each that still finds it so.
+    Without it lengths stay as they are, and a missing unfinished page counts
+    as given back: the sequence goes on in a free page whose first tokens are
+    another sequence's, for callers whose window hides them.
 
     A sequence's token is appended (at position seq_lens[r], which then grows
     by one) before it is forked again: a page taken for a token that never came
@@ -179,7 +188,8 @@ def fork_sequences(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: 
     # lengths and counts that go back, then the kernels' scratch
     lens, counts, scratch = ref_counts.new_empty(4 * rows + 3).split_with_sizes((rows, 3, 3 * rows))
     with _device_guard(device):
-        _lib.check(_lib.load().pa_fork_sequences(
+        lib = _lib.load()
+        _lib.check((lib.pa_fork_held_sequences if all_held else lib.pa_fork_sequences)(
             ptr, layer_stride, layers, page_stride, page_bytes, pages, block_tables.data_ptr(),
             _row_stride(block_tables), width, seq_lens.data_ptr(), parents.data_ptr(), rows,
             _page_size(kv_pool, kv_layout), ref_counts.data_ptr(), out.data_ptr(), _row_stride(out),

@@ -85,10 +85,15 @@ def test_release_leaves_a_row_past_its_table(pages, fi, lir):
 
 
 # ---------------------------------------------------------- sequences that have ended
-def plain_fork(tables, lens, refs, parents):
+def plain_fork(tables, lens, refs, parents, all_held=False):
     """(tables, lens, refs, counts, copies), with -1 for a parent of none."""
     rows, width = tables.shape
-    refs, out, out_lens = refs.copy(), np.full_like(tables, -1), np.zeros_like(lens)
+    lens, refs, out = lens.copy(), refs.copy(), np.full_like(tables, -1)
+    out_lens, lost = np.zeros_like(lens), set()
+    for s in range(rows):
+        if all_held and lens[s] % P and tables[s, lens[s] // P] < 0:
+            lost.add(s)
+            lens[s] = lens[s] // P * P
     for r in range(rows):
         for page in tables[r, :-(-lens[r] // P)]:
             if page >= 0:
@@ -106,14 +111,14 @@ def plain_fork(tables, lens, refs, parents):
     kept, wants, missing = set(), [], 0
     for r in alive:
         at = out_lens[r] // P
-        if r in last and last[r] not in held | kept:
+        if parents[r] in lost or at >= width:
+            missing += 1
+        elif r in last and last[r] not in held | kept:
             kept.add(last[r])
             refs[last[r]] += 1
             out[r, at] = last[r]
-        elif at < width:
-            wants.append(r)
         else:
-            missing += 1
+            wants.append(r)
     free = [i for i in range(len(refs)) if refs[i] == 0]
     copies = []
     for r, page in zip(wants, free):
@@ -121,7 +126,10 @@ def plain_fork(tables, lens, refs, parents):
         refs[page] = 1
         if r in last:
             copies.append((last[r], page))
-    missing += max(len(wants) - len(free), 0)
+    for r in wants[len(free):]:
+        missing += 1
+        if all_held:
+            out_lens[r] = out_lens[r] // P * P
     return out, out_lens, refs, [len(copies), min(len(wants), len(free)), missing], copies
 
 
@@ -222,3 +230,117 @@ def test_active_is_checked(fi):
                 torch.ones(2, 3, dtype=torch.bool, device=DEV), torch.ones(2, dtype=torch.bool)):
         with pytest.raises(ValueError, match="active"):
             beam.beam_search_step(x, s, _pool(4), t, n, c, active=bad)
+
+
+# ------------------------------------------------------------- pages that ran out
+def _fork_held(pages, fi, lir, pool, t, n, parents, c):
+    tables, lens, refs = (x.cpu().numpy().astype(np.int64) for x in (t, n, c))
+    want_t, want_l, want_r, want_c, copies = plain_fork(tables, lens, refs, parents, True)
+    want_pool = _copied(pool, copies)
+    with _status(fi, lir, lir._lib.PA_ERR_DEVICE_CHECK if want_c[2] else 0):
+        t, n, counts = pages.fork_sequences(pool, t, n, _i32(parents), c, all_held=True)
+        assert counts.tolist() == want_c
+    assert np.array_equal(t.cpu().numpy(), want_t) and np.array_equal(n.cpu().numpy(), want_l)
+    assert np.array_equal(c.cpu().numpy(), want_r)
+    assert torch.equal(_bits(pool), _bits(want_pool))
+    return t, n, want_c
+
+
+def test_forks_after_a_fork_that_found_no_page(pages, fi, lir):
+    """The lost tokens are counted in every fork, never replaced by the tokens
+    of a free page."""
+    t, n, c = _i32([[0, 1, -1], [2, 3, -1]]), _i32([20, 20]), _i32([1, 1, 1, 1])
+    pool = _pool(4, 2, 1, 8)
+    c[1] += 1  # row 0's unfinished page has another holder: it needs a copy
+    t, n, counts = _fork_held(pages, fi, lir, pool, t, n, np.array([0, 1]), c)
+    assert counts == [0, 0, 1] and n.tolist() == [16, 20] and t.tolist()[0] == [0, -1, -1]
+    # pages are free again, the caller counts a token that had no page
+    c = torch.cat([c, torch.zeros(4, dtype=torch.int32, device=DEV)])
+    pool = torch.cat([pool, _pool(4, 2, 1, 8, seed=1)], 1)
+    for _ in range(2):
+        t, n, counts = _fork_held(pages, fi, lir, pool, t, n + 1, np.array([0, 1]), c)
+        assert counts[2] == 1 and n[0] == 16 and t[0].tolist() == [0, -1, -1]
+    # not counted, the row goes on from its full pages
+    n[1] += 1
+    t, n, counts = _fork_held(pages, fi, lir, pool, t, n, np.array([0, 1]), c)
+    assert counts == [0, 1, 0] and n[0] == 16 and t[0, 1] >= 0
+    # another row continues a lost one: it shares the full page and is counted
+    t[0, 1] = -1
+    n[0] = 18
+    t, n, counts = _fork_held(pages, fi, lir, pool, t, n, np.array([0, 0]), c)
+    assert counts[2] == 2 and n.tolist() == [16, 16] and c[0] == 2
+
+
+def crowded(seed, rows, steps=5):
+    """Tables, lengths, counts, the pages that others hold (half of them), and
+    for each step parents and which rows have a token counted for which there
+    was no page."""
+    rng = np.random.RandomState(1000 * seed + rows)
+    lens = rng.randint(0, 60, rows)
+    need = sum(-(-x // P) for x in lens)
+    tables = np.full((rows, 6), -1, dtype=np.int64)
+    ids = rng.permutation(need + rows // 16).tolist()
+    for r in range(rows):
+        for j in range(-(-lens[r] // P)):
+            tables[r, j] = ids.pop()
+    others = (rng.rand(need + rows // 16) < 0.5).astype(np.int64)
+    others[ids] = 0
+    refs = others.copy()
+    np.add.at(refs, tables[tables >= 0], 1)
+    plan = []
+    for _ in range(steps):
+        parents = np.where(rng.rand(rows) < 0.8, np.arange(rows), rng.randint(0, rows, rows))
+        parents[rng.rand(rows) < 0.05] = -1
+        plan.append((parents, rng.rand(rows) < 0.5))
+    return tables, lens, refs, others, plan
+
+
+def tokens_to_come(tables, lens, parents, anyway):
+    """Which rows' lengths grow after a fork."""
+    width = tables.shape[1]
+    at = np.minimum(lens // P, width - 1)
+    has = tables[np.arange(len(lens)), at] >= 0
+    return (has | anyway) & (parents >= 0) & (lens < P * width)
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("rows", [12, 60, 1100])
+def test_forks_in_a_pool_that_is_too_small(pages, fi, lir, seed, rows):
+    """Random steps, some rows ending, more pages wanted than there are; what
+    the lengths count is always in pages that the counts hold."""
+    tables, lens, refs, others, plan = crowded(seed, rows)
+    t, n, c, pool = _i32(tables), _i32(lens), _i32(refs), _pool(len(refs), 1, 1, 8)
+    short = 0
+    for parents, anyway in plan:
+        t, n, counts = _fork_held(pages, fi, lir, pool, t, n, parents, c)
+        short += counts[2]
+        assert torch.equal(c, _references(t, len(refs)) + _i32(others))
+        tables, lens = t.cpu().numpy(), n.cpu().numpy()
+        for r in range(rows):
+            assert (tables[r, :-(-lens[r] // P)] >= 0).all()
+        n = n + _i32(tokens_to_come(tables, lens, parents, anyway))
+    assert short > 0
+
+
+def test_a_beam_search_step_reports_a_lost_page_until_the_beam_ends(fi, lir):
+    beam = importlib.import_module("llm-inference-runtime_b200.beam")
+    t, n = _i32([[0, 1, -1], [0, 2, -1]]), _i32([20, 20])
+    c, pool = _i32([2, 2, 1]), _pool(3, 1, 1, 8)
+    scores = torch.zeros(1, 2, device=DEV)
+    # (apart by far: each beam goes on with itself)
+    logits = torch.zeros(1, 2, 50, device=DEV)
+    logits[0, 0, 7] = logits[0, 1, 9] = 60.0
+    for step in range(3):
+        with _status(fi, lir, lir._lib.PA_ERR_DEVICE_CHECK):
+            got = beam.beam_search_step(logits, scores, pool, t, n, c)
+            assert got["parents"].tolist() == [[0, 1]] and got["counts"].tolist() == [0, 0, 1]
+        t, n, scores = got["block_tables"], got["seq_lens"], got["scores"]
+        assert n.tolist() == [16, 20 + step] and t[0].tolist() == [0, -1, -1]
+        n = n + 1
+        if step == 0:  # there would be a page now
+            c = torch.cat([c, torch.zeros(2, dtype=torch.int32, device=DEV)])
+            pool = torch.cat([pool, _pool(2, 1, 1, 8, seed=1)], 1)
+    with _status(fi, lir, 0):
+        got = beam.beam_search_step(logits, scores, pool, t, n, c,
+                                    active=torch.tensor([False], device=DEV))
+        assert (got["block_tables"] == -1).all() and c.tolist() == [0, 1, 0, 0, 0]
