@@ -288,8 +288,9 @@ int pa_compact_pages(void* pool, int64_t layer_stride_bytes, int32_t num_layers,
  *   scores[b, w] + (logits[b, w, v] - lse),  lse = log sum_v exp(logits[b, w, v])
  * (lse rounded to fp32, the sum of the three ordered in fp64). The
  * num_candidates <= 32 best of a request (num_beams <= 256, vocab_size <=
- * 2^24, batch_size <= 65535), best first; equal scores by the lowest beam, inside a beam by the
- * larger logit, then the lowest token: out_scores (fp32), out_parents
+ * 2^24, batch_size * num_beams < 2^31), best first; equal scores by the lowest
+ * beam, inside a beam by the larger logit, then the lowest token: out_scores
+ * (fp32), out_parents
  * (b * num_beams + w, a row of pa_fork_sequences), out_tokens, each
  * [batch, num_candidates].
  * A NaN logit counts as -inf, +inf as its type's largest value; beams whose

@@ -22,7 +22,7 @@ _DTYPES = {torch.float16: _lib.PA_DTYPE_F16, torch.bfloat16: _lib.PA_DTYPE_BF16,
 MAX_CANDIDATES = 32
 MAX_BEAMS = 256
 MAX_VOCAB = 2 ** 24
-MAX_BATCH = 65535
+MAX_ROWS = 2 ** 31 - 1  # of all requests' beams
 
 
 @functools.lru_cache(maxsize=256)
@@ -43,7 +43,7 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
     [batch, num_candidates], best first; equal scores by the lowest beam,
     inside a beam by the larger logit, then the lowest token. parents are
     rows ``b * beams + w``, as ``pages.fork_sequences`` takes them. A NaN
-    logit counts as -inf."""
+    logit counts as -inf. At most 32 candidates of 256 beams."""
     if logits.dim() != 3 or scores.dim() != 2 or logits.shape[:2] != scores.shape:
         raise ValueError("logits must be [batch, beams, vocab] and scores [batch, beams]")
     if logits.dtype not in _DTYPES:
@@ -56,9 +56,10 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
     n = int(num_candidates)
     if beams == 0 or vocab == 0 or not 1 <= n <= beams * vocab:
         raise ValueError("num_candidates must be in [1, beams * vocab]")
-    if n > MAX_CANDIDATES or beams > MAX_BEAMS or vocab > MAX_VOCAB or batch > MAX_BATCH:
+    if (n > MAX_CANDIDATES or beams > MAX_BEAMS or vocab > MAX_VOCAB
+            or batch * beams > MAX_ROWS):
         raise NotImplementedError(f"at most {MAX_CANDIDATES} candidates of {MAX_BEAMS} beams and "
-                                  f"{MAX_VOCAB} tokens, {MAX_BATCH} requests")
+                                  f"{MAX_VOCAB} tokens, {MAX_ROWS} beams in all")
     if vocab > 1 and logits.stride(2) != 1:
         raise ValueError("the vocabulary dimension of logits must be contiguous")
     if scores.size(1) > 1 and scores.stride(1) != 1:
@@ -86,7 +87,8 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, kv_pool: torch.
                      ref_counts: torch.Tensor, kv_layout: str = "HND",
                      active: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
     """One step of beam search: each request's beams are replaced by its
-    ``beams`` best continuations and their cache follows.
+    ``beams`` best continuations and their cache follows. As many candidates
+    as beams are selected, so there are at most 32 beams here.
 
     Row ``b * beams + w`` of ``block_tables`` / ``seq_lens`` is beam w of
     request b. Returns scores, parents and tokens [batch, beams] and the new

@@ -678,9 +678,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(const BeamParam
     });
   __syncthreads();
   auto put = [&](int k, const JoinKey& c) {
-    p.out_scores[b * K + k] = static_cast<float>(order_value64(c.score));
-    p.out_parents[b * K + k] = b * p.beams + 255 - static_cast<int>(c.rest >> 56);
-    p.out_tokens[b * K + k] = 0xffffff - static_cast<int>(c.rest & 0xffffff);
+    const int64_t at = static_cast<int64_t>(b) * K + k;
+    p.out_scores[at] = static_cast<float>(order_value64(c.score));
+    p.out_parents[at] = b * p.beams + 255 - static_cast<int>(c.rest >> 56);
+    p.out_tokens[at] = 0xffffff - static_cast<int>(c.rest & 0xffffff);
   };
   const int n = s_n;
   if (n <= kBeamCap) {

@@ -860,6 +860,8 @@ int check_beam(int batch, int beams, int vocab, int k, int dtype) {
   const int64_t flat = static_cast<int64_t>(beams) * vocab;
   if (k > flat) return PA_ERR_INVALID_ARGUMENT;
   if (k > kBeamMaxK || beams > kBeamMaxBeams || vocab > kBeamMaxVocab) return PA_ERR_UNSUPPORTED;
+  // a row's number is an int32 of the output and a block of the grid's first dimension
+  if (static_cast<int64_t>(batch) * beams > 0x7fffffffLL) return PA_ERR_UNSUPPORTED;
   return PA_OK;
 }
 
@@ -895,7 +897,6 @@ int pa_beam_select(const void* logits, int64_t logits_stride_b, int64_t logits_s
   const int sms = sm_count(dev) > 0 ? sm_count(dev) : 148;
   const int64_t rows = static_cast<int64_t>(batch_size) * num_beams;
   const BeamCut cut = beam_cut(dtype, batch_size, num_beams, vocab_size, num_candidates, sms);
-  if (batch_size > 65535) return PA_ERR_UNSUPPORTED;  // the grid's third dimension
   const BeamWsLayout L = beam_ws_layout(rows, cut.chunks, num_candidates);
   if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
   uint8_t* ws = static_cast<uint8_t*>(workspace);

@@ -43,3 +43,18 @@ def test_a_step_checks_which_requests_go_on(lir):
     for bad in (torch.ones(2), torch.ones(3, dtype=torch.bool), torch.ones(2, 3, dtype=torch.bool)):
         with pytest.raises(ValueError, match="active"):
             beam.beam_search_step(x, s, pool, t, n, n, active=bad)
+
+
+def test_rows_of_a_selection_are_counted_together(lib, lir):
+    """As many requests as give 2^31 - 1 beams pass (the workspace is looked at
+    next), one more beam is refused."""
+    E = lir._lib
+
+    def call(batch, beams):
+        return lib.pa_beam_select(D, 400, 100, D, 4, batch, beams, 100, 8, E.PA_DTYPE_F32, D, D, D, D,
+                                  100, None)
+
+    for batch, beams in ((65536, 4), (2 ** 31 - 1, 1), (2 ** 23 - 1, 256)):
+        assert call(batch, beams) == E.PA_ERR_WORKSPACE_TOO_SMALL, (batch, beams)
+    for batch, beams in ((2 ** 23, 256), (2 ** 30, 2)):
+        assert call(batch, beams) == E.PA_ERR_UNSUPPORTED, (batch, beams)
