@@ -37,7 +37,7 @@ def _on_gpu_i32(t: torch.Tensor, name: str, dim: int) -> torch.Tensor:
         raise TypeError(f"{name} must be int32")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
-    if t.dim() != dim or (t.stride()[-1] != 1 and t.numel() > 0):
+    if t.dim() != dim or (t.shape[-1] > 1 and t.stride()[-1] != 1):
         raise ValueError(f"{name} must be {dim}-D with contiguous entries")
     return t
 

@@ -39,6 +39,27 @@ def test_select_for_many_requests(beam, dtype, batch):
     assert torch.equal(parents, want_p[which] + shift[:, None])
 
 
+def test_tensors_of_one_entry_have_any_stride(pages):
+    """One sequence, one page: views whose only entry has no neighbour."""
+    one = lambda v: torch.tensor([[v, 9], [9, 9]], dtype=torch.int32, device=DEV)[:1, 0]  # noqa: E731
+    assert one(3).stride() == (2,)
+    tables, lens, refs = _i32([[0]]), one(P), one(1)
+    counts = pages.free_sequences(tables, lens, refs)
+    assert counts.tolist() == [1, 1, 0] and tables.tolist() == [[-1]]
+    assert lens.tolist() == [0] and refs.tolist() == [0]
+    # a column of a table, row after row
+    wide = _i32([[0, 5], [1, 5], [2, 5]])
+    t, n, c = wide[:, :1], _i32([P, 3, 0]), _i32([1, 1, 1])
+    assert pages.evict_window_pages(t, n, c, 0).tolist() == [0, 0, 0]
+    refs = one(1)
+    remap, counts = pages.compact_pages(_pool(1), _i32([[0]]), one(P), refs)
+    assert remap.tolist() == [0] and counts.tolist() == [1, 0, 0]
+    t, n, counts = pages.fork_sequences(_pool(1), _i32([[0]]), one(5), one(0), one(1))
+    assert t.tolist() == [[0]] and n.tolist() == [5] and counts.tolist() == [0, 0, 0]
+    with pytest.raises(ValueError, match="contiguous"):
+        pages.free_sequences(_i32([[0], [1]]), _i32([[1, 0], [1, 0]])[:, 0], _i32([1, 1]))
+
+
 def test_beams_at_their_limits(beam, pages):
     """32 beams step, 256 beams select, one more of each is refused."""
     logits, scores = _random(1, 256, 40, torch.float32, seed=3)
