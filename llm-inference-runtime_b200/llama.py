@@ -120,25 +120,25 @@ def init_flashinfer_state(*, kv_pool: torch.Tensor, page_size: int, device,
     last ``window_left + 1`` tokens plus the first ``num_sink_tokens``
     (not in the reference); pages behind it can be given back between steps
     with ``pages.evict_window_pages``."""
+    ws = torch.empty(WORKSPACE_BYTES, dtype=torch.uint8, device=device)
+    if window_left is None:
+        if num_sink_tokens:
+            raise ValueError("num_sink_tokens needs a window_left")
+        prefill = flashinfer.BatchPrefillWithPagedKVCacheWrapper(ws, "HND")
+        decode = flashinfer.BatchDecodeWithPagedKVCacheWrapper(ws, "HND")
+    else:
+        window = {"window_left": window_left, "num_sink_tokens": num_sink_tokens}
+        prefill = flashinfer.BatchPrefillWithSlidingWindowWrapper(ws, "HND", **window)
+        decode = flashinfer.BatchDecodeWithSlidingWindowWrapper(ws, "HND", **window)
+    # what can be refused was: a refused call leaves the state as it was
     PagedAttnState.kv_pool = kv_pool
     PagedAttnState.page_size = page_size
     PagedAttnState.dtype = kv_pool.dtype
     PagedAttnState.window_left = window_left
     PagedAttnState.num_sink_tokens = num_sink_tokens
-    PagedAttnState.workspace_buffer = torch.empty(WORKSPACE_BYTES, dtype=torch.uint8,
-                                                  device=device)
-    ws = PagedAttnState.workspace_buffer
-    if window_left is None:
-        if num_sink_tokens:
-            raise ValueError("num_sink_tokens needs a window_left")
-        PagedAttnState.prefill_wrapper = flashinfer.BatchPrefillWithPagedKVCacheWrapper(ws, "HND")
-        PagedAttnState.decode_wrapper = flashinfer.BatchDecodeWithPagedKVCacheWrapper(ws, "HND")
-        return
-    window = {"window_left": window_left, "num_sink_tokens": num_sink_tokens}
-    PagedAttnState.prefill_wrapper = flashinfer.BatchPrefillWithSlidingWindowWrapper(
-        ws, "HND", **window)
-    PagedAttnState.decode_wrapper = flashinfer.BatchDecodeWithSlidingWindowWrapper(
-        ws, "HND", **window)
+    PagedAttnState.workspace_buffer = ws
+    PagedAttnState.prefill_wrapper = prefill
+    PagedAttnState.decode_wrapper = decode
 
 
 init_paged_attn_state = init_flashinfer_state
