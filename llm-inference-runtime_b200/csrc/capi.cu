@@ -1131,6 +1131,7 @@ struct DecodeAppend {
 // table arguments of decode_run are then the plan's compacted table.
 struct DecodeWindow {
   int4 key;
+  size_t table_bytes;
   const int4* window;
   const int32_t* table_indptr;
   const int32_t* table_indices;
@@ -1158,7 +1159,8 @@ int decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h, const pa_k
   const int dev = current_device();
   DecodePlanShape sh;
   if (!decode_shape(dev, hkv, D, &sh)) return dev < 0 ? PA_ERR_CUDA : PA_ERR_UNSUPPORTED;
-  const DecodeWsLayout L = decode_ws_layout(sh.units, batch_size, hkv, D, sh.g.hb);
+  const DecodeWsLayout L = decode_ws_layout(sh.units, batch_size, hkv, D, sh.g.hb,
+                                            win != nullptr ? win->table_bytes : 0);
   if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
   CUtensorMap km, vm;
   if ((st = encode_kv_map(&km, cache->k_base, *cache, kPage, sh.g.hb)) != PA_OK) return st;
@@ -1342,12 +1344,12 @@ int window_decode_run(const void* q, int64_t q_stride_n, int64_t q_stride_h,
   if (L.total > workspace_bytes) return PA_ERR_WORKSPACE_TOO_SMALL;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const DecodeWindow win{
-      window_plan_key(window_left, num_sink_tokens, L.capacity, num_kv_indices),
+      window_plan_key(window_left, num_sink_tokens, L.capacity, num_kv_indices), L.table_bytes,
       reinterpret_cast<const int4*>(ws + L.window), kv_indptr, kv_indices};
   return decode_run(q, q_stride_n, q_stride_h, cache,
                     reinterpret_cast<const int32_t*>(ws + L.indices),
                     reinterpret_cast<const int32_t*>(ws + L.indptr), kv_last_page_len, batch_size,
-                    num_qo_heads, sm_scale, ws, L.indptr, out, lse, stream, app, &win);
+                    num_qo_heads, sm_scale, ws, workspace_bytes, out, lse, stream, app, &win);
 }
 
 }  // namespace

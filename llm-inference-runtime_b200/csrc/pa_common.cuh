@@ -55,13 +55,15 @@ struct DecodeWsLayout {
   size_t hdr, unit_start, empty, counter, part_lse, part_o, total;
 };
 
+// table_bytes (a multiple of 256) behind the header are left to the caller.
 __host__ __device__ inline DecodeWsLayout decode_ws_layout(int num_units, int batch, int hkv,
-                                                           int head_dim, int heads_per_unit) {
+                                                           int head_dim, int heads_per_unit,
+                                                           size_t table_bytes = 0) {
   DecodeWsLayout L;
   const size_t slots = static_cast<size_t>(num_units) * 2 * heads_per_unit;
   size_t o = 0;
   L.hdr = o;
-  o = align256(o + sizeof(DecodePlanHeader));
+  o = align256(o + sizeof(DecodePlanHeader)) + table_bytes;
   L.unit_start = o;  // int4 {b, head block, j, 0} of each group's first page
   o = align256(o + sizeof(int4) * static_cast<size_t>(num_units));
   L.empty = o;  // int32 list of requests without pages

@@ -50,11 +50,13 @@ __host__ __device__ inline WindowSpan window_span(int64_t first_query, int windo
   return w;
 }
 
-// Workspace of a window decode: the decode plan, whose header is at offset 0 as
-// every plan's is, then the compacted table. A plan of any other kind over the
-// same workspace so replaces the header, whatever else it leaves standing.
+// Workspace of a window decode: the decode plan's, with the compacted table
+// between its header and the rest. The header is at offset 0 as every plan's
+// is, so a plan of any other kind over the same workspace replaces it, whatever
+// else it leaves standing. (Behind the plan's partial states, megabytes away,
+// the table cost each launch 0.4 us.)
 struct WindowDecodeWsLayout {
-  size_t indptr, window, indices, total;
+  size_t indptr, window, indices, table_bytes, total;
   int64_t capacity;  // page ids the compacted table holds
 };
 
@@ -79,14 +81,17 @@ __host__ __device__ inline WindowDecodeWsLayout window_decode_ws_layout(
   WindowDecodeWsLayout L;
   const int64_t most = window_pages_max(window, sinks, page_size) * batch;
   L.capacity = most < num_indices ? most : num_indices;
-  size_t o = decode_bytes;
+  constexpr size_t kHeader = 256;
+  static_assert(sizeof(DecodePlanHeader) <= kHeader, "the table starts at the next 256 bytes");
+  size_t o = kHeader;
   L.indptr = o;
   o = align256(o + 4 * (static_cast<size_t>(batch) + 1));
   L.window = o;  // int4 {hole_lo, hole_hi, sink_pages, shift} per request
   o = align256(o + sizeof(int4) * static_cast<size_t>(batch));
   L.indices = o;
   o = align256(o + 4 * static_cast<size_t>(L.capacity));
-  L.total = o;
+  L.table_bytes = o - kHeader;
+  L.total = decode_bytes + L.table_bytes;
   return L;
 }
 
@@ -197,7 +202,8 @@ __global__ void __launch_bounds__(kWindowPlanThreads)
     }
     decode_plan_block(FreshIndptr{s_held, out_indptr}, last_len, batch, hkv, hq, head_dim, page_size,
                       L.capacity, num_groups, hb, min_per_group, ws, kWindowDecodeMagic, s_bad != 0,
-                      max_pieces, window_plan_key(window, sinks, L.capacity, num_indices));
+                      max_pieces, window_plan_key(window, sinks, L.capacity, num_indices),
+                      L.table_bytes);
     return;
   }
   int32_t* out_indices = reinterpret_cast<int32_t*>(ws + L.indices);
