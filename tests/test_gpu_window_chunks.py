@@ -83,3 +83,27 @@ def test_scores_of_full_batches(fi, dtype, batch, beams, vocab):
     assert np.array_equal(tokens[some].cpu().numpy(), want_t)
     off = np.abs(best[some].cpu().double().numpy() - want)
     assert (off <= near + 2.0 ** -24 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("rows", [2047, 2048, 2049, 5000])
+def test_decode_plans_of_more_requests_than_the_plan_keeps_at_hand(fi, rows):
+    """The plan's own table is read back from memory past its first entries."""
+    kv = np.random.RandomState(rows).randint(0, 60, rows).tolist()
+    kv[-1], kv[rows // 2] = 700, 333
+    pr = Problem([1] * rows, kv, 4, 1, 64, 24, 3, seed=rows)
+    w = fi.BatchDecodeWithSlidingWindowWrapper(_ws(), "HND", window_left=24, num_sink_tokens=3)
+    w.plan(_t(pr.indptr), _t(pr.indices), _t(pr.last), 4, 1, 64, P, q_data_type=pr.dtype)
+    pr.check(*w.run(pr.q.to(DEV), pr.device_pool(), return_lse=True))
+
+
+@pytest.mark.parametrize("rows", [63, 64, 65, 300, 1100])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill_of_many_requests(fi, rows, causal):
+    """Around the number of requests from which the plan gives a thread, not a
+    warp, to each."""
+    rng = np.random.RandomState(rows)
+    qo = rng.randint(0, 4, rows)
+    kv = qo + rng.randint(0, 60, rows)
+    qo[rows // 3], kv[rows // 3] = 260, 900
+    pr = Problem(qo.tolist(), kv.tolist(), 8, 2, 64, 33, 5, seed=rows, causal=causal)
+    pr.check(*_prefill(fi, pr))
