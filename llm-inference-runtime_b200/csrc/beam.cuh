@@ -21,11 +21,14 @@
 // their two largest maxima searched, which every thread keeps in shared memory
 // (all their logits are read again if a third step reaches it too), and what
 // passes is ranked by counting. (Reading the step again instead of keeping it
-// took 3 us of a CTA's 19, now 0.9.) Many threads
-// reach it only when many logits are equal to it (masked or constant rows):
-// then the ones above it and, in index order, as many equal ones as are missing
-// are taken. If more than kBeamCap lie above it (a layout against the threads'
-// order), K rounds of a block-wide maximum give the same result.
+// took 3 us of a CTA's 19, now 0.9.) Many threads reach it only when many
+// logits are equal to it (masked or constant rows): then the ones above it and,
+// in index order, as many equal ones as are missing are taken, from memory
+// again. So a vocabulary masked down to fewer than K tokens a chunk, by -inf or
+// by a finite mask, is read three times (64 x 8 beams over 128256, bf16: 36.7 us
+// unmasked, 37.8 with 1 in 100 tokens left, 81 with 16 of them). If more than
+// kBeamCap lie above it (a layout against the threads' order), K rounds of a
+// block-wide maximum give the same result.
 #pragma once
 
 #include "pa_common.cuh"

@@ -812,9 +812,22 @@ namespace {
 // its threads hold: 8 beams of one request over 128256 bf16 logits take 18.1
 // us in 32 chunks a row, 12.5 in 16 and 10.2 in 8. Where that leaves many
 // places free (few chunks a row) each row gets one more, shorter chunk; these
-// start last and fill the places in turn while the others still run: 64 such
-// requests take 37.9 us with one chunk a row, 37.6 with two halves, 37.3 so;
-// over 50257 tokens 31.0 with halves, 26.7 so.
+// start last and fill the places in turn while the others still run.
+//
+// Device time of a call from a CUDA graph, us, bf16, 8 beams and 16 candidates,
+// equal chunks -> with the shorter one; 740 places:
+//   rows  full       32000         50257        128256 tokens
+//    192     3   12.7 -> 14.4  16.9 -> 16.5  20.4 -> 22.0
+//    256     2   14.2 -> 14.9  20.1 -> 18.4  25.4 -> 25.2
+//    368     2   15.9 -> 16.0  21.4 -> 21.3  30.6 -> 30.4
+//    512     1   18.1 -> 18.7  29.0 -> 25.8  39.5 -> 36.6
+//    600     1   20.3 -> 18.8  31.0 -> 28.9  44.0 -> 39.4
+// (600: 150 x 4 beams, 8 candidates.) `rounds` one less than come to a place,
+// against as many and two less: 512 rows over 50257 tokens 25.8, 26.5 and 30.5,
+// over 128256 36.6, 37.6 and 37.2; 600 rows over 128256 39.4, 44.0 and 39.6. With
+// rounds up to 2 only, those 600 rows stay at 44.2; 640 rows (6 rounds) stay at
+// 46.6 with this limit and would take 42.7 without, 736 rows (4 places free) 48.4
+// either way.
 struct BeamCut {
   int chunks, vectors;
 };

@@ -39,7 +39,9 @@ namespace pa {
 
 // Two non-negative fp32 values -> packed 16-bit pair (lo in the low half).
 // Both types: the hardware round-to-nearest-even conversion, one instruction
-// per pair.
+// per pair. The MMA takes P in V's type: half a step per probability, against
+// sums kept in fp32 (bf16 outputs 0.0023 relative off fp64 instead of the 0.0017
+// of their own rounding).
 template <typename T>
 __device__ __forceinline__ uint32_t pack_p(float lo, float hi);
 template <>
@@ -202,6 +204,7 @@ __global__ void prefill_plan_kernel(const int32_t* __restrict__ qo_indptr,
     const int n = kv_indptr[b + 1] - kv_indptr[b];
     return n > 0 ? (n - 1) * page_size + last_len[b] : 0;
   };
+  // (of a causal launch; of another one it only orders the items)
   auto cost_of = [&](int qo_len, int kv_len, int t0) {
     int end = min(kv_len, kv_len - qo_len + t0 + qt);
     if (window >= 0)  // (window < 0: none)
@@ -782,9 +785,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const int key0 = j * kPfKeys;
       if constexpr (kWindow) {
         // Hidden: columns >= e, and columns [a, b). Both as one bit mask per
-        // 32 columns, and only where a row of the warp hides some of them: a
-        // tile's 128 comparisons with each end took 147 us where this takes
-        // 141 (16 chunks of 512 rows, window 1024, 32 heads of 128).
+        // 32 columns, and only where a row of the warp hides some of them: with
+        // a tile's 128 comparisons with each end plan and run take 135.1 us from
+        // a CUDA graph, so 129.0 (16 chunks of 512 rows, window 1024, 32 heads
+        // of 128).
         const int a = p.sinks - key0, b = hole_hi - key0, e = lim - key0;
         if (!__all_sync(0xffffffffu, e >= kPfKeys && b <= 0)) {
           auto below = [](int x) {  // bits 0 .. x - 1
