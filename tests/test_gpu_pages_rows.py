@@ -344,3 +344,45 @@ def test_a_beam_search_step_reports_a_lost_page_until_the_beam_ends(fi, lir):
         got = beam.beam_search_step(logits, scores, pool, t, n, c,
                                     active=torch.tensor([False], device=DEV))
         assert (got["block_tables"] == -1).all() and c.tolist() == [0, 1, 0, 0, 0]
+
+
+def test_steps_captured_and_replayed_while_requests_end(fi, lir):
+    """One graph of a step; which requests go on changes between replays."""
+    beam = importlib.import_module("llm-inference-runtime_b200.beam")
+    batch, beams, vocab, total = 4, 2, 300, 40
+    rows, length = batch * beams, P + 5
+    tables = torch.arange(rows * 2, device=DEV).view(rows, 2).int()
+    t, n = torch.cat([tables, torch.full_like(tables, -1)], 1), _i32(np.full(rows, length))
+    refs = _references(t, total)
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(batch, beams, vocab, generator=g).to(DEV)
+    s = -torch.rand(batch, beams, generator=g).to(DEV)
+    active = torch.ones(batch, dtype=torch.bool, device=DEV)
+    c, fresh = refs.clone(), _pool(total, 2, 1, 8)
+    pool = fresh.clone()
+    with _status(fi, lir, 0):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            beam.beam_search_step(x, s, fresh.clone(), t, n, refs.clone(), active=active)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = beam.beam_search_step(x, s, pool, t, n, c, active=active)
+        for on in ([1, 1, 1, 1], [1, 0, 1, 0], [0, 0, 0, 0], [0, 1, 1, 1]):
+            active.copy_(torch.tensor(on, dtype=torch.bool))
+            x.copy_(torch.randn(batch, beams, vocab, generator=g))
+            c.copy_(refs)
+            pool.copy_(fresh)
+            graph.replay()
+            _, choice, _ = beam.beam_search_select(x, s, beams)
+            parents = choice.masked_fill(~active[:, None], -1).view(-1).cpu().numpy()
+            want_t, want_l, want_r, want_c, copies = plain_fork(
+                t.cpu().numpy().astype(np.int64), n.cpu().numpy().astype(np.int64),
+                refs.cpu().numpy().astype(np.int64), parents, True)
+            assert got["parents"].view(-1).tolist() == parents.tolist()
+            assert got["counts"].tolist() == want_c
+            assert np.array_equal(got["block_tables"].cpu().numpy(), want_t)
+            assert np.array_equal(got["seq_lens"].cpu().numpy(), want_l)
+            assert np.array_equal(c.cpu().numpy(), want_r)
+            assert torch.equal(_bits(pool), _bits(_copied(fresh, copies)))
